@@ -12,6 +12,8 @@ Device-tensor entry points (torch tensors on a CUDA device):
     attention(q, k, v, causal=..., ...)      -> tcgen05 kernel (bf16/f16) or fp32 kernel
     lse_merge_(o_acc, lse_acc, o_part, lse_part)
     quantize_rows_int8(x), attention_int8(...), int8_logits(...)
+    paged_append, paged_attention, attention_key_weights, paged_evict: the
+        paged key-value cache of single-token attention (kv_cache.py)
 Host drop-ins of the crate (numpy / sequences of float, fp32):
     waller_operator, waller_operator_parallel, standard_attention
 Scalar helpers of the crate (pure host logic, not the hot path):
@@ -142,6 +144,7 @@ def lib():
     L.gae_debug_attn_trace.argtypes = [vp, C.c_int]
     L.gae_debug_wait_timeout.argtypes = [C.c_uint64, vp]
     L.gae_debug_attn_int8_logits.argtypes = [C.POINTER(AttnInt8Args), vp, vp]
+    _kv_bind(L)
     _lib = L
     return L
 
@@ -874,3 +877,10 @@ def symphony_forward(x, k, v, w_up, w_down, norm1_w, norm2_w, tuning: TuningFork
                                   C.byref(tuning), out.data_ptr(), workspace.data_ptr(),
                                   workspace.numel(), _stream_ptr(stream)))
     return out
+
+
+# ------------------------------------------------- paged key-value cache
+from .kv_cache import (KeyWeightsArgs, KvPool, PagedAppendArgs, PagedAttnArgs,  # noqa: E402
+                       PagedEvictArgs, attention_key_weights, paged_append, paged_attention,
+                       paged_evict)
+from .kv_cache import _bind as _kv_bind  # noqa: E402

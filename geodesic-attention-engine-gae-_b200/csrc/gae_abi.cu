@@ -22,6 +22,8 @@
 #include "layer_sm100.cuh"
 #include "symphony.cuh"
 #include "crate_f32.cuh"
+#include "kv_cache.cuh"
+#include "key_weights.cuh"
 
 namespace {
 
@@ -821,6 +823,7 @@ bool mul_ok(size_t a, size_t b, size_t *out) { return !__builtin_mul_overflow(a,
 }  // namespace
 
 #include "ring.cuh"
+#include "kv_cache_abi.cuh"
 
 // ==================================================================== C ABI
 extern "C" {

@@ -1,0 +1,251 @@
+// kv_cache_abi.cuh -- the C ABI of the paged key-value cache and of the key
+// weights: argument checks and launches.  Included by gae_abi.cu after its
+// helpers (fail, set_smem, num_sms): one translation unit.
+#pragma once
+
+namespace {
+
+int dtype_size(gae_dtype t) { return t == GAE_DTYPE_F32 ? 4 : t == GAE_DTYPE_BF16 || t == GAE_DTYPE_F16 ? 2 : 0; }
+
+// Strides that keep every row on a 16-byte boundary.
+bool row_strides(const int64_t *s, int n, int esize) {
+    for (int i = 0; i < n; ++i)
+        if (s[i] < 0 || (s[i] * esize) % 16) return false;
+    return true;
+}
+
+// Fits an int with room for one page more (positions are 32-bit, rows 64-bit).
+constexpr int64_t kMaxPositions = 1ll << 30;
+
+gae_status check_pool(const gae_kv_pool *pl, gae::KvPool *out) {
+    if (!pl) return fail(GAE_ERR_INVALID_ARG, "pool is NULL");
+    const int es = dtype_size(pl->dtype);
+    if (!es) return fail(GAE_ERR_INVALID_ARG, "unknown dtype %d", (int)pl->dtype);
+    if (pl->num_pages < 0 || pl->kv_heads < 1 || pl->page_size < 1 || pl->head_dim < 1)
+        return fail(GAE_ERR_INVALID_ARG, "invalid pool shape [%lld, %lld, %lld, %lld]", (long long)pl->num_pages,
+                    (long long)pl->kv_heads, (long long)pl->page_size, (long long)pl->head_dim);
+    if (pl->num_pages > INT32_MAX || pl->kv_heads > 65535 || pl->page_size > kMaxPositions)
+        return fail(GAE_ERR_UNSUPPORTED, "pool beyond 2^31 - 1 pages, 65535 heads or 2^30 rows to a page");
+    if (pl->head_dim > 256 || (pl->head_dim * es) % 16)
+        return fail(GAE_ERR_UNSUPPORTED, "the cache needs head_dim <= 256 in rows of a multiple of 16 bytes, got %lld",
+                    (long long)pl->head_dim);
+    if (pl->num_pages > 0 && (!pl->k || !pl->v)) return fail(GAE_ERR_INVALID_ARG, "pool pointers are NULL");
+    if (!aligned16(pl->k) || !aligned16(pl->v)) return fail(GAE_ERR_INVALID_ARG, "pools must be 16-byte aligned");
+    if (!row_strides(pl->k_stride, 3, es) || !row_strides(pl->v_stride, 3, es))
+        return fail(GAE_ERR_INVALID_ARG, "pool strides must be non-negative multiples of 16 bytes");
+    out->k = pl->k; out->v = pl->v;
+    out->k_sp = pl->k_stride[0]; out->k_sh = pl->k_stride[1]; out->k_ss = pl->k_stride[2];
+    out->v_sp = pl->v_stride[0]; out->v_sh = pl->v_stride[1]; out->v_ss = pl->v_stride[2];
+    out->num_pages = pl->num_pages;
+    out->Hkv = (int)pl->kv_heads; out->page = (int)pl->page_size; out->D = (int)pl->head_dim;
+    return GAE_OK;
+}
+
+gae_status check_table(const int32_t *entry, int64_t stride, int64_t max_pages, int64_t batch, int64_t page,
+                       gae::PageTable *out) {
+    if (max_pages < 0 || stride < 0) return fail(GAE_ERR_INVALID_ARG, "negative page table size or stride");
+    if (max_pages > 0 && !entry) return fail(GAE_ERR_INVALID_ARG, "page table is NULL");
+    if (max_pages > kMaxPositions / page)
+        return fail(GAE_ERR_UNSUPPORTED, "a page table of more than 2^30 positions");
+    out->entry = entry; out->stride = stride; out->max_pages = (int)max_pages;
+    return GAE_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+gae_status gae_paged_append(const gae_kv_pool *pool, const gae_paged_append_args *a, void *stream) {
+    gae::AppendParams p;
+    memset(&p, 0, sizeof(p));
+    gae_status s;
+    if ((s = check_pool(pool, &p.pool)) != GAE_OK) return s;
+    if (!a) return fail(GAE_ERR_INVALID_ARG, "args is NULL");
+    if (a->batch < 0 || a->tokens < 0) return fail(GAE_ERR_INVALID_ARG, "negative batch or tokens");
+    if ((s = check_table(a->page_table, a->table_stride, a->max_pages, a->batch, pool->page_size, &p.table)) != GAE_OK)
+        return s;
+    if (a->batch == 0 || a->tokens == 0) return GAE_OK;
+    const int es = dtype_size(pool->dtype);
+    if (!a->k_new || !a->v_new || !a->start) return fail(GAE_ERR_INVALID_ARG, "NULL pointer in append arguments");
+    if (!aligned16(a->k_new) || !aligned16(a->v_new) || !row_strides(a->k_new_stride, 3, es) ||
+        !row_strides(a->v_new_stride, 3, es))
+        return fail(GAE_ERR_INVALID_ARG, "new rows must be 16-byte aligned, with non-negative strides of 16 bytes");
+    if (a->batch > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch > 65535");
+    p.k_new = a->k_new; p.v_new = a->v_new;
+    p.kn_sb = a->k_new_stride[0]; p.kn_sh = a->k_new_stride[1]; p.kn_st = a->k_new_stride[2];
+    p.vn_sb = a->v_new_stride[0]; p.vn_sh = a->v_new_stride[1]; p.vn_st = a->v_new_stride[2];
+    p.start = a->start; p.counts = a->counts;
+    p.chunks = (int)(pool->head_dim * es / 16);
+    if (a->tokens > kMaxPositions) return fail(GAE_ERR_UNSUPPORTED, "more than 2^30 new tokens");
+    p.tokens = (int)a->tokens;
+    const int64_t blocks = (a->tokens * p.chunks * pool->kv_heads + 255) / 256;
+    if (blocks > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many new rows");
+    const dim3 grid((unsigned)blocks, (unsigned)a->batch);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (es == 4) gae::paged_append_kernel<4><<<grid, 256, 0, st>>>(p);
+    else gae::paged_append_kernel<2><<<grid, 256, 0, st>>>(p);
+    GAE_CUDA_TRY(cudaGetLastError());
+    return GAE_OK;
+}
+
+size_t gae_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                      int64_t capacity, int with_weights) {
+    if (batch < 1 || heads < 1 || kv_heads < 1 || head_dim < 1 || capacity < 0 || batch > 65535 || heads > 65535 ||
+        capacity > kMaxPositions)
+        return 0;
+    if (!with_weights) return 0;
+    return (size_t)batch * heads * (capacity + 1) * 4;
+}
+
+gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args *a, void *stream) {
+    gae::PagedAttnParams p;
+    memset(&p, 0, sizeof(p));
+    gae_status s;
+    if ((s = check_pool(pool, &p.pool)) != GAE_OK) return s;
+    if (!a) return fail(GAE_ERR_INVALID_ARG, "args is NULL");
+    if (a->batch < 0 || a->heads < 1) return fail(GAE_ERR_INVALID_ARG, "invalid batch or heads");
+    if (a->heads % pool->kv_heads) return fail(GAE_ERR_INVALID_ARG, "heads must be a multiple of kv_heads");
+    if ((s = check_table(a->page_table, a->table_stride, a->max_pages, a->batch, pool->page_size, &p.table)) != GAE_OK)
+        return s;
+    if (a->batch == 0) return GAE_OK;
+    if (a->batch > 65535 || a->heads > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch or heads > 65535");
+    const int es = dtype_size(pool->dtype);
+    if (!a->q || !a->o || !a->seq_lens) return fail(GAE_ERR_INVALID_ARG, "NULL pointer in paged attention arguments");
+    if (!aligned16(a->q) || !aligned16(a->o) || !row_strides(a->q_stride, 2, es) || !row_strides(a->o_stride, 2, es))
+        return fail(GAE_ERR_INVALID_ARG, "q and o must be 16-byte aligned, with non-negative strides of 16 bytes");
+    if (!(a->scale >= 0.f)) return fail(GAE_ERR_UNSUPPORTED, "negative or NaN scale");
+    if ((a->weights != nullptr) != (a->weights_out != nullptr))
+        return fail(GAE_ERR_INVALID_ARG, "weights and weights_out go together");
+    if (a->weights_out && (a->w_stride[0] < 0 || a->w_stride[1] < 0 || a->w_out_stride[0] < 0 || a->w_out_stride[1] < 0))
+        return fail(GAE_ERR_INVALID_ARG, "negative weights stride");
+    const int64_t cap = a->max_pages * pool->page_size;
+    if (a->weights_out && a->weights_len < cap)
+        return fail(GAE_ERR_INVALID_ARG, "weights rows of %lld entries for %lld positions", (long long)a->weights_len,
+                    (long long)cap);
+    const size_t need =
+        gae_paged_attn_workspace_bytes(a->batch, a->heads, pool->kv_heads, pool->head_dim, cap, a->weights_out != nullptr);
+    if (need && (!a->workspace || !aligned16(a->workspace)))
+        return fail(GAE_ERR_INVALID_ARG, "workspace is NULL or not 16-byte aligned");
+    if (a->workspace_bytes < need)
+        return fail(GAE_ERR_INVALID_ARG, "workspace too small: %zu < %zu", a->workspace_bytes, need);
+    p.q = a->q; p.o = a->o; p.lse = a->lse; p.lens = a->seq_lens;
+    p.q_sb = a->q_stride[0]; p.q_sh = a->q_stride[1]; p.o_sb = a->o_stride[0]; p.o_sh = a->o_stride[1];
+    p.B = (int)a->batch; p.H = (int)a->heads; p.cap = (int)cap;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->weights_out) {
+        p.scores = static_cast<float *>(a->workspace);
+        if (!p.lse) p.lse = p.scores + (size_t)a->batch * a->heads * cap;
+        p.w_in = a->weights; p.w_out = a->weights_out;
+        p.wi_sb = a->w_stride[0]; p.wi_sh = a->w_stride[1];
+        p.wo_sb = a->w_out_stride[0]; p.wo_sh = a->w_out_stride[1];
+    }
+    const dim3 grid((unsigned)a->heads, (unsigned)a->batch);
+    switch (pool->dtype) {
+        case GAE_DTYPE_F32: gae::paged_attn_kernel<float><<<grid, 128, 0, st>>>(p); break;
+        case GAE_DTYPE_BF16: gae::paged_attn_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p); break;
+        case GAE_DTYPE_F16: gae::paged_attn_kernel<__half><<<grid, 128, 0, st>>>(p); break;
+    }
+    GAE_CUDA_TRY(cudaGetLastError());
+    if (a->weights_out && cap > 0) {
+        const dim3 g2((unsigned)((cap + 255) / 256), (unsigned)pool->kv_heads, (unsigned)a->batch);
+        gae::paged_weights_kernel<<<g2, 256, 0, st>>>(p);
+        GAE_CUDA_TRY(cudaGetLastError());
+    }
+    return GAE_OK;
+}
+
+size_t gae_key_weights_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv) {
+    (void)batch; (void)heads; (void)kv_heads; (void)seq_q; (void)seq_kv;
+    return 0;
+}
+
+gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
+    if (!a) return fail(GAE_ERR_INVALID_ARG, "args is NULL");
+    if (a->batch < 1 || a->heads < 1 || a->kv_heads < 1 || a->seq_q < 0 || a->seq_kv < 0 || a->head_dim < 1)
+        return fail(GAE_ERR_INVALID_ARG, "invalid key weights shape");
+    if (a->heads % a->kv_heads) return fail(GAE_ERR_INVALID_ARG, "heads must be a multiple of kv_heads");
+    if (a->head_dim != 64 && a->head_dim != 128)
+        return fail(GAE_ERR_UNSUPPORTED, "key weights support head_dim 64 or 128, got %lld", (long long)a->head_dim);
+    if (a->dtype != GAE_DTYPE_BF16 && a->dtype != GAE_DTYPE_F16)
+        return fail(GAE_ERR_UNSUPPORTED, "key weights support bf16 and f16");
+    if (a->batch * a->heads > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch*heads > 65535");
+    if (a->seq_q > kMaxPositions || a->seq_kv > kMaxPositions)
+        return fail(GAE_ERR_UNSUPPORTED, "sequence longer than 2^30");
+    if (!(a->scale >= 0.f)) return fail(GAE_ERR_UNSUPPORTED, "negative or NaN scale");
+    if (a->seq_kv == 0) return GAE_OK;
+    if (!a->out || (a->seq_q > 0 && (!a->q || !a->k || !a->lse)))
+        return fail(GAE_ERR_INVALID_ARG, "NULL pointer in key weights arguments");
+    if (!aligned16(a->q) || !aligned16(a->k) || !row_strides(a->q_stride, 3, 2) || !row_strides(a->k_stride, 3, 2))
+        return fail(GAE_ERR_INVALID_ARG, "q and k must be 16-byte aligned, with non-negative strides of 16 bytes");
+    for (int i = 0; i < 2; ++i)
+        if (a->lse_stride[i] < 0 || a->out_stride[i] < 0)
+            return fail(GAE_ERR_INVALID_ARG, "negative lse or out stride");
+    gae::KeyWeightsParams p;
+    memset(&p, 0, sizeof(p));
+    p.q = a->q; p.k = a->k; p.lse = a->lse; p.out = a->out;
+    p.q_sb = a->q_stride[0]; p.q_sh = a->q_stride[1]; p.q_ss = a->q_stride[2];
+    p.k_sb = a->k_stride[0]; p.k_sh = a->k_stride[1]; p.k_ss = a->k_stride[2];
+    p.l_sb = a->lse_stride[0]; p.l_sh = a->lse_stride[1];
+    p.o_sb = a->out_stride[0]; p.o_sh = a->out_stride[1];
+    p.B = (int)a->batch; p.H = (int)a->heads; p.Hkv = (int)a->kv_heads;
+    p.Nq = (int)a->seq_q; p.Nkv = (int)a->seq_kv; p.D = (int)a->head_dim;
+    p.causal = a->causal ? 1 : 0;
+    p.accumulate = a->accumulate ? 1 : 0;
+    p.off = a->q_offset - a->kv_offset;
+    p.scale_log2 = a->scale * 1.4426950408889634f;
+    const dim3 grid((unsigned)((a->seq_kv + 63) / 64), (unsigned)a->kv_heads, (unsigned)a->batch);
+    const int smem = 2 * 64 * (p.D + 1) * 4;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    gae_status s;
+    if (a->dtype == GAE_DTYPE_BF16) {
+        if ((s = set_smem(gae::key_weights_kernel<__nv_bfloat16>, smem)) != GAE_OK) return s;
+        gae::key_weights_kernel<__nv_bfloat16><<<grid, 256, smem, st>>>(p);
+    } else {
+        if ((s = set_smem(gae::key_weights_kernel<__half>, smem)) != GAE_OK) return s;
+        gae::key_weights_kernel<__half><<<grid, 256, smem, st>>>(p);
+    }
+    GAE_CUDA_TRY(cudaGetLastError());
+    return GAE_OK;
+}
+
+gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *a, void *stream) {
+    gae::EvictParams p;
+    memset(&p, 0, sizeof(p));
+    gae_status s;
+    if ((s = check_pool(pool, &p.pool)) != GAE_OK) return s;
+    if (!a) return fail(GAE_ERR_INVALID_ARG, "args is NULL");
+    if (a->batch < 0) return fail(GAE_ERR_INVALID_ARG, "negative batch");
+    if ((s = check_table(a->page_table, a->table_stride, a->max_pages, a->batch, pool->page_size, &p.src)) != GAE_OK ||
+        (s = check_table(a->dst_table, a->dst_stride, a->dst_max_pages, a->batch, pool->page_size, &p.dst)) != GAE_OK)
+        return s;
+    if (a->keep < 1 || a->recent < 0 || a->recent > a->keep)
+        return fail(GAE_ERR_INVALID_ARG, "eviction needs 1 <= keep and 0 <= recent <= keep, got %lld and %lld",
+                    (long long)a->keep, (long long)a->recent);
+    if (a->keep > a->dst_max_pages * pool->page_size)
+        return fail(GAE_ERR_INVALID_ARG, "dst_table has room for %lld positions, keep is %lld",
+                    (long long)(a->dst_max_pages * pool->page_size), (long long)a->keep);
+    if (a->batch == 0) return GAE_OK;
+    if (a->batch > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch > 65535");
+    if (!a->seq_lens || !a->new_lens || !a->kept || !a->kept_weights || (a->max_pages > 0 && a->weights_len > 0 && !a->weights))
+        return fail(GAE_ERR_INVALID_ARG, "NULL pointer in eviction arguments");
+    if (a->page_table == a->dst_table) return fail(GAE_ERR_INVALID_ARG, "dst_table must name other pages than page_table");
+    if (a->w_stride[0] < 0 || a->w_stride[1] < 0 || a->weights_len < 0)
+        return fail(GAE_ERR_INVALID_ARG, "negative weights stride or length");
+    p.lens = a->seq_lens; p.w = a->weights;
+    p.w_sb = a->w_stride[0]; p.w_sh = a->w_stride[1];
+    p.keep = (int)a->keep; p.recent = (int)a->recent; p.cap = (int)gae::min64(a->max_pages * pool->page_size, a->weights_len);
+    p.new_lens = a->new_lens; p.kept = a->kept; p.w_out = a->kept_weights;
+    const int es = dtype_size(pool->dtype);
+    p.chunks = (int)(pool->head_dim * es / 16);
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    gae::evict_select_kernel<<<dim3((unsigned)pool->kv_heads, (unsigned)a->batch), 1024, 0, st>>>(p);
+    GAE_CUDA_TRY(cudaGetLastError());
+    const dim3 grid((unsigned)((a->keep * p.chunks + 255) / 256), (unsigned)pool->kv_heads, (unsigned)a->batch);
+    if (es == 4) gae::evict_gather_kernel<4><<<grid, 256, 0, st>>>(p);
+    else gae::evict_gather_kernel<2><<<grid, 256, 0, st>>>(p);
+    GAE_CUDA_TRY(cudaGetLastError());
+    return GAE_OK;
+}
+
+}  // extern "C"

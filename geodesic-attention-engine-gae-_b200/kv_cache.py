@@ -1,0 +1,306 @@
+"""Paged key-value cache: device-tensor entry points and the cache of a model.
+
+The reference crate attends whole sequences only; this is the serving side of
+its operator: new rows are written to pages (paged_append), one new token per
+sequence attends over them (paged_attention), and a cache is brought back to a
+budget by the attention weight its keys have drawn (attention_key_weights for a
+prompt, paged_attention's own sums while decoding, paged_evict).
+
+Pools are [num_pages, kv_heads, page_size, head_dim] tensors (strided views
+allowed, the head_dim contiguous); a page table is int32 [batch, max_pages] and
+position t of sequence b is slot t % page_size of page table[b, t // page_size].
+An entry outside [0, num_pages) holds no keys.
+
+Every function runs on `stream` (default: the current stream of the tensors'
+device), allocates what it returns and its workspace there, never synchronises
+and may be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes as C
+import math
+
+from . import GAEError, _check, _dtype_code, _torch, lib
+
+_I64_2, _I64_3 = C.c_int64 * 2, C.c_int64 * 3
+
+
+class KvPool(C.Structure):
+    """Mirror of gae_kv_pool (include/gae.h)."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", _I64_3), ("v_stride", _I64_3),
+                ("num_pages", C.c_int64), ("kv_heads", C.c_int64), ("page_size", C.c_int64),
+                ("head_dim", C.c_int64), ("dtype", C.c_int)]
+
+
+class PagedAppendArgs(C.Structure):
+    """Mirror of gae_paged_append_args (include/gae.h)."""
+    _fields_ = [("k_new", C.c_void_p), ("v_new", C.c_void_p), ("k_new_stride", _I64_3),
+                ("v_new_stride", _I64_3), ("batch", C.c_int64), ("tokens", C.c_int64),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int64),
+                ("start", C.c_void_p), ("counts", C.c_void_p)]
+
+
+class PagedAttnArgs(C.Structure):
+    """Mirror of gae_paged_attn_args (include/gae.h)."""
+    _fields_ = [("q", C.c_void_p), ("o", C.c_void_p), ("lse", C.c_void_p), ("q_stride", _I64_2),
+                ("o_stride", _I64_2), ("batch", C.c_int64), ("heads", C.c_int64),
+                ("page_table", C.c_void_p), ("table_stride", C.c_int64), ("max_pages", C.c_int64),
+                ("seq_lens", C.c_void_p), ("scale", C.c_float), ("weights", C.c_void_p),
+                ("weights_out", C.c_void_p), ("w_stride", _I64_2), ("w_out_stride", _I64_2),
+                ("weights_len", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class KeyWeightsArgs(C.Structure):
+    """Mirror of gae_key_weights_args (include/gae.h)."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("lse", C.c_void_p), ("out", C.c_void_p),
+                ("batch", C.c_int64), ("heads", C.c_int64), ("kv_heads", C.c_int64),
+                ("seq_q", C.c_int64), ("seq_kv", C.c_int64), ("head_dim", C.c_int64),
+                ("q_stride", _I64_3), ("k_stride", _I64_3), ("lse_stride", _I64_2),
+                ("out_stride", _I64_2), ("dtype", C.c_int), ("causal", C.c_int),
+                ("accumulate", C.c_int), ("scale", C.c_float), ("q_offset", C.c_int64),
+                ("kv_offset", C.c_int64), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
+
+
+class PagedEvictArgs(C.Structure):
+    """Mirror of gae_paged_evict_args (include/gae.h)."""
+    _fields_ = [("batch", C.c_int64), ("page_table", C.c_void_p), ("table_stride", C.c_int64),
+                ("max_pages", C.c_int64), ("seq_lens", C.c_void_p), ("weights", C.c_void_p),
+                ("w_stride", _I64_2), ("weights_len", C.c_int64), ("dst_table", C.c_void_p), ("dst_stride", C.c_int64),
+                ("dst_max_pages", C.c_int64), ("keep", C.c_int64), ("recent", C.c_int64),
+                ("new_lens", C.c_void_p), ("kept", C.c_void_p), ("kept_weights", C.c_void_p)]
+
+
+def _bind(L):
+    vp, i64, sz = C.c_void_p, C.c_int64, C.c_size_t
+    for name in ("gae_paged_append", "gae_paged_attn_fwd", "gae_paged_evict"):
+        getattr(L, name).argtypes = [vp, vp, vp]
+    L.gae_paged_attn_workspace_bytes.restype = sz
+    L.gae_paged_attn_workspace_bytes.argtypes = [i64, i64, i64, i64, i64, C.c_int]
+    L.gae_key_weights_workspace_bytes.restype = sz
+    L.gae_key_weights_workspace_bytes.argtypes = [i64] * 5
+    L.gae_key_weights.argtypes = [vp, vp]
+
+
+def _run(device, stream, tensors, body):
+    """body(stream pointer) with the tensors' device and `stream` current, so that
+    what it allocates belongs to the stream it runs on; on a stream other than
+    the current one the inputs are marked as used there."""
+    torch = _torch()
+    if stream is None and torch.cuda.current_device() == device.index:
+        return body(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device):
+        if stream is None:
+            return body(torch.cuda.current_stream().cuda_stream)
+        if stream.device != device:
+            raise GAEError(1, f"stream on {stream.device}, tensors on {device}")
+        with torch.cuda.stream(stream):
+            for t in tensors:
+                if t is not None:
+                    t.record_stream(stream)
+            return body(stream.cuda_stream)
+
+
+def _same_device(what, device, **tensors):
+    if device.type != "cuda":
+        raise GAEError(1, f"{what}: tensors must be on a CUDA device")
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise GAEError(1, f"{what}: {name} is on {t.device}, not {device}")
+
+
+def _pool(what, k_pages, v_pages):
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise GAEError(1, f"{what}: k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
+    if v_pages.dtype != k_pages.dtype:
+        raise GAEError(1, f"{what}: k_pages and v_pages must share a dtype")
+    ks, vs = k_pages.stride(), v_pages.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise GAEError(1, f"{what}: pages must have a contiguous head_dim")
+    return KvPool(k_pages.data_ptr(), v_pages.data_ptr(), _I64_3(*ks[:3]), _I64_3(*vs[:3]), *k_pages.shape,
+                  _dtype_code(k_pages))
+
+
+def _table(what, table, batch, name="page_table"):
+    if table.dim() != 2 or table.shape[0] != batch or table.dtype != _torch().int32 or \
+            (table.shape[1] > 1 and table.stride(1) != 1):
+        raise GAEError(1, f"{what}: {name} must be int32 [batch, max_pages] with contiguous rows")
+    return table.data_ptr(), table.stride(0), table.shape[1]
+
+
+def _ints(what, t, batch, name):
+    if t.dim() != 1 or t.shape[0] != batch or t.dtype != _torch().int32 or not t.is_contiguous():
+        raise GAEError(1, f"{what}: {name} must be contiguous int32 [batch]")
+    return t.data_ptr()
+
+
+def _weights(what, t, batch, heads, n, name):
+    if t.dim() != 3 or t.shape[0] != batch or t.shape[1] != heads or t.shape[2] < n or \
+            t.dtype != _torch().float32 or (t.shape[2] > 1 and t.stride(2) != 1):
+        raise GAEError(1, f"{what}: {name} must be fp32 [{batch}, {heads}, >= {n}] with contiguous rows")
+    return t.data_ptr(), _I64_2(t.stride(0), t.stride(1))
+
+
+def paged_append(k_new, v_new, k_pages, v_pages, page_table, start, *, counts=None, stream=None):
+    """Writes new rows into the cache: k_new/v_new [B, Hkv, T, D] (strided views
+    allowed); token t < counts[b] of sequence b (counts int32 [B], default T)
+    becomes position start[b] + t.  Tokens beyond the page table, or whose entry
+    names no page, are dropped."""
+    what = "paged_append"
+    if k_new.dim() != 4 or v_new.shape != k_new.shape:
+        raise GAEError(1, f"{what}: k_new and v_new must be [batch, kv_heads, tokens, head_dim]")
+    B, H, T, D = k_new.shape
+    if k_pages.dim() != 4 or k_pages.shape[1] != H or k_pages.shape[3] != D:
+        raise GAEError(1, f"{what}: k_new and k_pages differ in heads or head_dim")
+    if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
+        raise GAEError(1, f"{what}: new rows and pages must share a dtype")
+    pool = _pool(what, k_pages, v_pages)
+    ks, vs = k_new.stride(), v_new.stride()
+    if ks[3] != 1 or vs[3] != 1:
+        raise GAEError(1, f"{what}: new rows must have a contiguous head_dim")
+    a = PagedAppendArgs(k_new.data_ptr(), v_new.data_ptr(), _I64_3(*ks[:3]), _I64_3(*vs[:3]), B, T,
+                        *_table(what, page_table, B), _ints(what, start, B, "start"),
+                        None if counts is None else _ints(what, counts, B, "counts"))
+    _same_device(what, k_pages.device, v_pages=v_pages, k_new=k_new, v_new=v_new, page_table=page_table,
+                 start=start, counts=counts)
+    _run(k_pages.device, stream, (k_new, v_new, k_pages, v_pages, page_table, start, counts),
+         lambda st: _check(lib().gae_paged_append(C.byref(pool), C.byref(a), st)))
+
+
+def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, out=None, lse=None,
+                    return_lse=False, weights=None, weights_out=None, stream=None):
+    """Attention of one new token per sequence: q [B, H, D] over the first
+    seq_lens[b] cached positions (int32 [B]); H a multiple of the pages' heads.
+    bf16/f16/f32, any head_dim <= 256 in 16-byte multiples.  An empty sequence
+    gives 0 and lse -inf.
+
+    weights (fp32 [B, Hkv, >= the page table's positions]) asks for the keys'
+    attention weight: weights_out = weights + the softmax summed over each key head's
+    query heads; weights_out defaults to weights (in place).  Positions without
+    a key are left as they are."""
+    what = "paged_attention"
+    torch = _torch()
+    if q.dim() != 3:
+        raise GAEError(1, f"{what}: q must be [batch, heads, head_dim]")
+    B, H, D = q.shape
+    pool = _pool(what, k_pages, v_pages)
+    if k_pages.shape[3] != D or k_pages.dtype != q.dtype:
+        raise GAEError(1, f"{what}: q and the pages differ in head_dim or dtype")
+    Hkv, page = k_pages.shape[1], k_pages.shape[2]
+    table = _table(what, page_table, B)
+    lens = _ints(what, seq_lens, B, "seq_lens")
+    if q.stride(2) != 1:
+        raise GAEError(1, f"{what}: q must have a contiguous head_dim")
+    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+        raise GAEError(1, f"{what}: out must be like q, with a contiguous head_dim")
+    if lse is not None and (lse.shape != (B, H) or lse.dtype != torch.float32 or not lse.is_contiguous()):
+        raise GAEError(1, f"{what}: lse must be contiguous fp32 [batch, heads]")
+    cap = table[2] * page
+    w = wo = None
+    w_st = wo_st = _I64_2(0, 0)
+    w_len = 0
+    if weights is not None:
+        weights_out = weights if weights_out is None else weights_out
+        w, w_st = _weights(what, weights, B, Hkv, cap, "weights")
+        wo, wo_st = _weights(what, weights_out, B, Hkv, cap, "weights_out")
+        w_len = cap
+    elif weights_out is not None:
+        raise GAEError(1, f"{what}: weights_out without weights")
+    dev = k_pages.device
+    _same_device(what, dev, q=q, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, out=out, lse=lse,
+                 weights=weights, weights_out=weights_out)
+    L = lib()
+
+    def body(st):
+        o, l = out, lse
+        if o is None:
+            o = torch.empty((B, H, D), dtype=q.dtype, device=dev)
+        if return_lse and l is None:
+            l = torch.empty((B, H), dtype=torch.float32, device=dev)
+        n = L.gae_paged_attn_workspace_bytes(B, H, Hkv, D, cap, w is not None)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        a = PagedAttnArgs(q.data_ptr(), o.data_ptr(), None if l is None else l.data_ptr(),
+                          _I64_2(q.stride(0), q.stride(1)), _I64_2(o.stride(0), o.stride(1)), B, H, *table, lens,
+                          1.0 / math.sqrt(D) if scale is None else scale, w, wo, w_st, wo_st, w_len,
+                          ws.data_ptr() if n else None, n)
+        _check(L.gae_paged_attn_fwd(C.byref(pool), C.byref(a), st))
+        return (o, l) if return_lse else o
+
+    return _run(dev, stream, (q, k_pages, v_pages, page_table, seq_lens, out, lse, weights, weights_out), body)
+
+
+def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv_offset=0, out=None,
+                          accumulate=False, stream=None):
+    """The attention weight that the queries put on each key: fp32 [B, Hkv, Nkv],
+    sum over the queries that see the key (and the query heads of its key head)
+    of exp(scale * <q, k> - lse).  q [B, H, Nq, D], k [B, Hkv, Nkv, D] (bf16/f16,
+    head_dim 64/128, strided views allowed), lse [B, H, Nq] as attention(...,
+    return_lse=True) gives it (contiguous rows).  A window of a prompt's last
+    queries is q[:, :, -n:], lse[:, :, -n:] with q_offset = N - n.  out may be a
+    view of a cache's weights; accumulate=True adds to it."""
+    what = "attention_key_weights"
+    torch = _torch()
+    if q.dim() != 4 or k.dim() != 4:
+        raise GAEError(1, f"{what}: q and k must be [batch, heads, seq, head_dim]")
+    B, H, Nq, D = q.shape
+    Hkv, Nkv = k.shape[1], k.shape[2]
+    if k.shape[0] != B or k.shape[3] != D or k.dtype != q.dtype:
+        raise GAEError(1, f"{what}: q and k differ in batch, head_dim or dtype")
+    if q.stride(3) != 1 or k.stride(3) != 1:
+        raise GAEError(1, f"{what}: q and k must have a contiguous head_dim")
+    if lse.shape != (B, H, Nq) or lse.dtype != torch.float32 or (Nq > 1 and lse.stride(2) != 1):
+        raise GAEError(1, f"{what}: lse must be fp32 [batch, heads, seq_q] with contiguous rows")
+    if accumulate and out is None:
+        raise GAEError(1, f"{what}: accumulate needs out")
+    if out is not None and out.shape != (B, Hkv, Nkv):
+        raise GAEError(1, f"{what}: out must be [{B}, {Hkv}, {Nkv}]")
+    dev = q.device
+    _same_device(what, dev, k=k, lse=lse, out=out)
+    L = lib()
+    scale = 1.0 / math.sqrt(D) if scale is None else scale
+
+    def body(st):
+        w = torch.empty((B, Hkv, Nkv), dtype=torch.float32, device=dev) if out is None else out
+        o, os_ = _weights(what, w, B, Hkv, Nkv, "out")
+        n = L.gae_key_weights_workspace_bytes(B, H, Hkv, Nq, Nkv)
+        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+        a = KeyWeightsArgs(q.data_ptr(), k.data_ptr(), lse.data_ptr(), o, B, H, Hkv, Nq, Nkv, D,
+                           _I64_3(*q.stride()[:3]), _I64_3(*k.stride()[:3]),
+                           _I64_2(lse.stride(0), lse.stride(1)), os_, _dtype_code(q), 1 if causal else 0,
+                           1 if accumulate else 0, scale, q_offset, kv_offset, ws.data_ptr() if n else None, n)
+        _check(L.gae_key_weights(C.byref(a), st))
+        return w
+
+    return _run(dev, stream, (q, k, lse, out), body)
+
+
+def paged_evict(k_pages, v_pages, page_table, seq_lens, weights, dst_table, *, keep, recent=0, stream=None):
+    """Brings every sequence to at most `keep` cached positions: per key head the
+    `recent` last positions and those of the largest weights (fp32 [B, Hkv, n];
+    a sequence is cut to n; equal weights: the lower position, NaN largest).  The kept
+    rows are copied in order to positions 0, 1, ... of dst_table, whose pages
+    must not be among those read.  Returns (new lengths int32 [B], kept
+    positions int32 [B, Hkv, keep], -1 beyond the length, their weights fp32,
+    0 beyond)."""
+    what = "paged_evict"
+    torch = _torch()
+    pool = _pool(what, k_pages, v_pages)
+    Hkv, B = k_pages.shape[1], page_table.shape[0]
+    table = _table(what, page_table, B)
+    dst = _table(what, dst_table, B, "dst_table")
+    lens = _ints(what, seq_lens, B, "seq_lens")
+    w, w_st = _weights(what, weights, B, Hkv, 0, "weights")
+    dev = k_pages.device
+    _same_device(what, dev, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, weights=weights,
+                 dst_table=dst_table)
+    keep, recent = int(keep), int(recent)
+
+    def body(st):
+        new_lens = torch.empty(B, dtype=torch.int32, device=dev)
+        kept = torch.empty((B, Hkv, max(keep, 0)), dtype=torch.int32, device=dev)
+        kept_w = torch.empty((B, Hkv, max(keep, 0)), dtype=torch.float32, device=dev)
+        a = PagedEvictArgs(B, *table, lens, w, w_st, weights.shape[2], *dst, keep, recent, new_lens.data_ptr(),
+                           kept.data_ptr(), kept_w.data_ptr())
+        _check(lib().gae_paged_evict(C.byref(pool), C.byref(a), st))
+        return new_lens, kept, kept_w
+
+    return _run(dev, stream, (k_pages, v_pages, page_table, seq_lens, weights, dst_table), body)

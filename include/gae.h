@@ -464,6 +464,153 @@ GAE_API gae_status gae_layernorm_fwd(const void *x, const void *res, void *sum_o
                              const float *gamma, const float *beta, int64_t rows,
                              int64_t d, float eps, void *stream);
 
+/* ------------------------------------------------------------------------
+ * Paged key-value cache (no reference counterpart: the crate attends whole
+ * sequences only).  Keys and values live in pools of pages,
+ * [num_pages, kv_heads, page_size, head_dim], addressed through element
+ * strides {page, head, slot} (the head_dim stride is 1).  Position t of
+ * sequence b is slot t % page_size of page page_table[b * table_stride +
+ * t / page_size], an int32 in device memory.  An entry outside
+ * [0, num_pages) holds no keys: attention and eviction pass over its
+ * positions, a write to them is dropped.  A sequence's capacity is
+ * max_pages * page_size positions; a length in device memory outside
+ * [0, capacity] counts as the nearer bound.
+ *
+ * bf16, f16 or f32, any head_dim <= 256 whose rows are a multiple of 16 bytes,
+ * any page_size >= 1, heads a multiple of kv_heads (query head h reads key
+ * head h / (heads / kv_heads)).  Pool, row and output pointers are 16-byte
+ * aligned and their strides non-negative multiples of 16 bytes.  Two
+ * sequences may share pages that are only read.  Every entry point works on
+ * the current device, allocates nothing and may be captured into a CUDA graph.
+ * ---------------------------------------------------------------------- */
+typedef struct {
+    void *k;
+    void *v;
+    int64_t k_stride[3];        /* element strides: page, head, slot */
+    int64_t v_stride[3];
+    int64_t num_pages, kv_heads, page_size, head_dim;
+    gae_dtype dtype;
+} gae_kv_pool;
+
+/* Writes new rows into the cache: token t < counts[b] of sequence b (k_new,
+ * v_new [batch, kv_heads, tokens, head_dim], strides {batch, head, token})
+ * becomes position start[b] + t.  counts NULL: all `tokens` of every sequence.
+ * Positions beyond the capacity (or negative) are dropped.  Two tokens of one
+ * call must not name the same row of the same page. */
+typedef struct {
+    const void *k_new;
+    const void *v_new;
+    int64_t k_new_stride[3];    /* element strides: batch, head, token */
+    int64_t v_new_stride[3];
+    int64_t batch, tokens;
+    const int32_t *page_table;
+    int64_t table_stride, max_pages;
+    const int32_t *start;       /* [batch] */
+    const int32_t *counts;      /* [batch], may be NULL */
+} gae_paged_append_args;
+
+GAE_API gae_status gae_paged_append(const gae_kv_pool *pool, const gae_paged_append_args *args, void *stream);
+
+/* Attention of one new token per sequence over the cache: o[b, h] =
+ * sum_t softmax_t(scale * <q[b, h], k_t>) v_t over t < seq_lens[b] (q, o
+ * [batch, heads, head_dim], strides {batch, head}); lse (optional, fp32,
+ * contiguous [batch, heads]) as in gae_attn_fwd.  A sequence with no keys has
+ * o = 0 and lse = -inf.  Statistics and accumulation in fp32.
+ * With weights_out (fp32 [batch, kv_heads, weights_len], strides
+ * {batch, head}) the call also adds up the weight of every key:
+ * weights_out[b, hk, t] = weights[b, hk, t] + sum over the group's heads of
+ * softmax_t; weights may be weights_out itself, entries of positions without a
+ * key are not written.  `workspace`: device memory, 16-byte aligned, of at
+ * least gae_paged_attn_workspace_bytes(..., max_pages * page_size,
+ * weights_out != NULL) bytes, not shared with a call that may run at the same
+ * time. */
+typedef struct {
+    const void *q;
+    void *o;
+    float *lse;                 /* may be NULL */
+    int64_t q_stride[2];        /* element strides: batch, head */
+    int64_t o_stride[2];
+    int64_t batch, heads;
+    const int32_t *page_table;
+    int64_t table_stride, max_pages;
+    const int32_t *seq_lens;    /* [batch] */
+    float scale;
+    const float *weights;       /* NULL without weights_out */
+    float *weights_out;         /* may be NULL */
+    int64_t w_stride[2];        /* element strides: batch, head */
+    int64_t w_out_stride[2];
+    int64_t weights_len;        /* entries of a row of weights and weights_out, >= max_pages * page_size */
+    void *workspace;
+    size_t workspace_bytes;
+} gae_paged_attn_args;
+
+GAE_API size_t gae_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
+                                              int64_t capacity, int with_weights);
+
+GAE_API gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args *args, void *stream);
+
+/* The weight that a block of queries puts on each key, from the forward's
+ * log-sum-exp: out[b, hk, j] (+)= sum over the heads h of key head hk and the
+ * queries i that see key j of exp(scale * <q_i, k_j> - lse[b, h, i]).  q
+ * [batch, heads, seq_q, head_dim], k [batch, kv_heads, seq_kv, head_dim] with
+ * strides {batch, head, seq}; lse and out fp32 with strides {batch, head}
+ * (contiguous rows).  Masks and offsets as in gae_attn_fwd; a query whose lse
+ * is -inf adds nothing.  accumulate != 0 adds to out instead of overwriting
+ * it.  bf16 or f16, head_dim 64 or 128, pointers of q and k 16-byte aligned
+ * and their strides non-negative multiples of 8 elements. */
+typedef struct {
+    const void *q;
+    const void *k;
+    const float *lse;
+    float *out;
+    int64_t batch, heads, kv_heads, seq_q, seq_kv, head_dim;
+    int64_t q_stride[3];        /* element strides: batch, head, seq */
+    int64_t k_stride[3];
+    int64_t lse_stride[2];      /* element strides: batch, head */
+    int64_t out_stride[2];
+    gae_dtype dtype;
+    int causal;
+    int accumulate;
+    float scale;
+    int64_t q_offset;
+    int64_t kv_offset;
+    void *workspace;
+    size_t workspace_bytes;
+} gae_key_weights_args;
+
+GAE_API size_t gae_key_weights_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q,
+                                               int64_t seq_kv);
+
+GAE_API gae_status gae_key_weights(const gae_key_weights_args *args, void *stream);
+
+/* Eviction to a budget: of each sequence and key head, the `recent` last
+ * positions and the positions of the largest weights (fp32 [batch, kv_heads,
+ * weights_len], strides {batch, head}) are kept, min(keep, keys) in
+ * all.  Equal weights: the lower position is kept; NaN counts as the largest.
+ * The kept rows are copied in their order to positions 0, 1, ... of dst_table,
+ * whose pages must not be among those that the call reads (a free page each;
+ * the old pages may be shared and stay as they are).  Outputs, contiguous:
+ * new_lens [batch], kept [batch, kv_heads, keep] (positions, -1 beyond the
+ * new length) and kept_weights [batch, kv_heads, keep] (0 beyond it).
+ * 1 <= keep <= dst_max_pages * page_size, 0 <= recent <= keep. */
+typedef struct {
+    int64_t batch;
+    const int32_t *page_table;
+    int64_t table_stride, max_pages;
+    const int32_t *seq_lens;    /* [batch] */
+    const float *weights;
+    int64_t w_stride[2];        /* element strides: batch, head */
+    int64_t weights_len;        /* entries of a row of weights; a longer sequence is cut to it */
+    const int32_t *dst_table;
+    int64_t dst_stride, dst_max_pages;
+    int64_t keep, recent;
+    int32_t *new_lens;
+    int32_t *kept;
+    float *kept_weights;
+} gae_paged_evict_args;
+
+GAE_API gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *args, void *stream);
+
 #ifdef __cplusplus
 }  /* extern "C" */
 #endif

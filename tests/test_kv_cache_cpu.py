@@ -1,0 +1,189 @@
+"""The paged key-value cache's refusals and ctypes mirrors, without a GPU: every
+call here is answered by the argument checks before anything is launched."""
+import ctypes as C
+import os
+import subprocess
+
+import pytest
+
+torch = pytest.importorskip("torch")
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+PTR = 1 << 20  # a 16-byte aligned address that no refused call reads
+INVALID, UNSUPPORTED = 1, 2
+
+STRUCTS = [("gae_kv_pool", "KvPool"), ("gae_paged_append_args", "PagedAppendArgs"),
+           ("gae_paged_attn_args", "PagedAttnArgs"), ("gae_key_weights_args", "KeyWeightsArgs"),
+           ("gae_paged_evict_args", "PagedEvictArgs")]
+
+
+def test_mirrors_match_the_header(gae, tmp_path):
+    lines = ['#include <stddef.h>', '#include <stdio.h>', '#include "gae.h"', "int main(void) {"]
+    for cname, pyname in STRUCTS:
+        lines.append(f'printf("{cname} size %zu\\n", sizeof({cname}));')
+        for field, _ in getattr(gae, pyname)._fields_:
+            lines.append(f'printf("{cname} {field} %zu\\n", offsetof({cname}, {field}));')
+    src, exe = tmp_path / "layout.c", tmp_path / "layout"
+    src.write_text("\n".join(lines + ["return 0; }"]))
+    subprocess.run(["gcc", "-I", os.path.join(ROOT, "include"), str(src), "-o", str(exe)], check=True)
+    got = {}
+    for line in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.splitlines():
+        cname, key, val = line.split()
+        got[(cname, key)] = int(val)
+    for cname, pyname in STRUCTS:
+        cls = getattr(gae, pyname)
+        assert C.sizeof(cls) == got[(cname, "size")], cname
+        for field, _ in cls._fields_:
+            assert getattr(cls, field).offset == got[(cname, field)], (cname, field)
+
+
+def _pool(gae, **kw):
+    s = gae.KvPool(PTR, PTR, (C.c_int64 * 3)(2 * 16 * 64, 16 * 64, 64), (C.c_int64 * 3)(2 * 16 * 64, 16 * 64, 64), 10, 2,
+                   16, 64, gae.DTYPE_BF16)
+    for k, v in kw.items():
+        if isinstance(v, tuple):
+            getattr(s, k)[:] = v
+        else:
+            setattr(s, k, v)
+    return s
+
+
+def _args(cls, base, **kw):
+    s = cls()
+    for k, v in {**base, **kw}.items():
+        if isinstance(v, tuple):
+            getattr(s, k)[:] = v
+        else:
+            setattr(s, k, v)
+    return s
+
+
+APPEND = dict(k_new=PTR, v_new=PTR, k_new_stride=(128, 64, 128), v_new_stride=(128, 64, 128), batch=1, tokens=1,
+              page_table=PTR, table_stride=4, max_pages=4, start=PTR)
+ATTN = dict(q=PTR, o=PTR, q_stride=(256, 64), o_stride=(256, 64), batch=1, heads=4, page_table=PTR, table_stride=4,
+            max_pages=4, seq_lens=PTR, scale=0.125, workspace=PTR, workspace_bytes=1 << 30)
+KEYS = dict(q=PTR, k=PTR, lse=PTR, out=PTR, batch=1, heads=4, kv_heads=2, seq_q=16, seq_kv=16, head_dim=64,
+            q_stride=(4096, 1024, 64), k_stride=(4096, 1024, 64), lse_stride=(64, 16), out_stride=(32, 16), dtype=1,
+            scale=0.125, workspace=PTR, workspace_bytes=1 << 30)
+EVICT = dict(batch=1, page_table=PTR, table_stride=4, max_pages=4, seq_lens=PTR, weights=PTR, w_stride=(128, 64),
+             weights_len=64, dst_table=PTR + 4096, dst_stride=2, dst_max_pages=2, keep=32, recent=4, new_lens=PTR,
+             kept=PTR, kept_weights=PTR)
+
+POOL_BAD = [(dict(num_pages=-1), INVALID), (dict(kv_heads=0), INVALID), (dict(page_size=0), INVALID),
+            (dict(head_dim=0), INVALID), (dict(head_dim=60), UNSUPPORTED), (dict(head_dim=264), UNSUPPORTED),
+            (dict(k=None), INVALID), (dict(v=PTR + 8), INVALID), (dict(k_stride=(2048, 1024, 60)), INVALID),
+            (dict(v_stride=(-2048, 1024, 64)), INVALID), (dict(dtype=7), INVALID),
+            (dict(num_pages=1 << 31), UNSUPPORTED), (dict(kv_heads=65536), UNSUPPORTED)]
+
+
+@pytest.mark.parametrize("bad,status", POOL_BAD)
+def test_pool_refusals(gae, bad, status):
+    L, pool = gae.lib(), _pool(gae, **bad)
+    for fn, cls, base in (("gae_paged_append", gae.PagedAppendArgs, APPEND),
+                          ("gae_paged_attn_fwd", gae.PagedAttnArgs, ATTN),
+                          ("gae_paged_evict", gae.PagedEvictArgs, EVICT)):
+        a = _args(cls, base, **({"heads": 65536 * 4} if "kv_heads" in bad and fn == "gae_paged_attn_fwd" else {}))
+        assert getattr(L, fn)(C.byref(pool), C.byref(a), None) == status, fn
+
+
+def _refused(gae, fn, cls, base, bad, status):
+    a = _args(cls, base, **bad)
+    assert getattr(gae.lib(), fn)(C.byref(_pool(gae)), C.byref(a), None) == status
+    assert gae.lib().gae_last_error(None, 0) == status
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(batch=-1), INVALID), (dict(tokens=-1), INVALID), (dict(k_new=None), INVALID), (dict(start=None), INVALID),
+    (dict(page_table=None), INVALID), (dict(max_pages=-1), INVALID), (dict(table_stride=-4), INVALID),
+    (dict(v_new=PTR + 2), INVALID), (dict(k_new_stride=(128, 60, 128)), INVALID),
+    (dict(v_new_stride=(128, 64, -128)), INVALID), (dict(batch=65536), UNSUPPORTED),
+    (dict(max_pages=1 << 30), UNSUPPORTED), (dict(tokens=(1 << 30) + 1), UNSUPPORTED)])
+def test_append_refusals(gae, bad, status):
+    _refused(gae, "gae_paged_append", gae.PagedAppendArgs, APPEND, bad, status)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(batch=-1), INVALID), (dict(heads=0), INVALID), (dict(heads=3), INVALID), (dict(q=None), INVALID),
+    (dict(o=PTR + 8), INVALID), (dict(seq_lens=None), INVALID), (dict(q_stride=(256, 60)), INVALID),
+    (dict(o_stride=(256, -64)), INVALID), (dict(scale=-1.0), UNSUPPORTED), (dict(scale=float("nan")), UNSUPPORTED),
+    (dict(weights=PTR), INVALID), (dict(weights_out=PTR), INVALID),
+    (dict(weights=PTR, weights_out=PTR, weights_len=63), INVALID),
+    (dict(weights=PTR, weights_out=PTR, weights_len=64, w_stride=(-1, 0)), INVALID),
+    (dict(weights=PTR, weights_out=PTR, weights_len=64, workspace_bytes=16), INVALID),
+    (dict(weights=PTR, weights_out=PTR, weights_len=64, workspace=None), INVALID),
+    (dict(batch=65536), UNSUPPORTED)])
+def test_attention_refusals(gae, bad, status):
+    _refused(gae, "gae_paged_attn_fwd", gae.PagedAttnArgs, ATTN, bad, status)
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(batch=0), INVALID), (dict(heads=3), INVALID), (dict(kv_heads=0), INVALID), (dict(seq_q=-1), INVALID),
+    (dict(head_dim=96), UNSUPPORTED), (dict(dtype=0), UNSUPPORTED), (dict(q=None), INVALID), (dict(out=None), INVALID),
+    (dict(k=PTR + 8), INVALID), (dict(k_stride=(4096, 1024, 60)), INVALID), (dict(lse_stride=(-1, 16)), INVALID),
+    (dict(scale=-0.5), UNSUPPORTED), (dict(batch=20000), UNSUPPORTED)])
+def test_key_weights_refusals(gae, bad, status):
+    a = _args(gae.KeyWeightsArgs, KEYS, **bad)
+    assert gae.lib().gae_key_weights(C.byref(a), None) == status
+
+
+@pytest.mark.parametrize("bad,status", [
+    (dict(batch=-1), INVALID), (dict(keep=0), INVALID), (dict(recent=-1), INVALID), (dict(recent=33), INVALID),
+    (dict(keep=33), INVALID), (dict(dst_table=PTR), INVALID), (dict(weights=None), INVALID), (dict(kept=None), INVALID),
+    (dict(seq_lens=None), INVALID), (dict(w_stride=(-1, 0)), INVALID), (dict(weights_len=-1), INVALID),
+    (dict(dst_table=None), INVALID), (dict(batch=65536), UNSUPPORTED)])
+def test_evict_refusals(gae, bad, status):
+    _refused(gae, "gae_paged_evict", gae.PagedEvictArgs, EVICT, bad, status)
+
+
+def test_null_structs(gae):
+    L, pool = gae.lib(), _pool(gae)
+    for fn in ("gae_paged_append", "gae_paged_attn_fwd", "gae_paged_evict"):
+        assert getattr(L, fn)(None, None, None) == INVALID
+        assert getattr(L, fn)(C.byref(pool), None, None) == INVALID
+    assert L.gae_key_weights(None, None) == INVALID
+
+
+def test_empty_calls_touch_nothing(gae):
+    L, pool = gae.lib(), _pool(gae)
+    for fn, cls, base in (("gae_paged_append", gae.PagedAppendArgs, APPEND),
+                          ("gae_paged_attn_fwd", gae.PagedAttnArgs, ATTN),
+                          ("gae_paged_evict", gae.PagedEvictArgs, EVICT)):
+        assert getattr(L, fn)(C.byref(pool), C.byref(_args(cls, base, batch=0)), None) == 0
+    assert L.gae_paged_append(C.byref(pool), C.byref(_args(gae.PagedAppendArgs, APPEND, tokens=0)), None) == 0
+    assert L.gae_key_weights(C.byref(_args(gae.KeyWeightsArgs, KEYS, seq_kv=0)), None) == 0
+
+
+def test_python_refusals(gae):
+    """The wrappers' own checks, on CPU tensors: shapes and types first, the device last."""
+    z = torch.zeros
+    k = z(4, 2, 16, 64, dtype=torch.bfloat16)
+    table, ints = z(3, 2, dtype=torch.int32), z(3, dtype=torch.int32)
+    new = z(3, 2, 5, 64, dtype=torch.bfloat16)
+    q = z(3, 4, 64, dtype=torch.bfloat16)
+    w = z(3, 2, 32)
+    append = lambda **s: gae.paged_append(**{**dict(k_new=new, v_new=new, k_pages=k, v_pages=k, page_table=table,  # noqa: E731
+                                                    start=ints), **s})
+    attend = lambda **s: gae.paged_attention(**{**dict(q=q, k_pages=k, v_pages=k, page_table=table,  # noqa: E731
+                                                       seq_lens=ints), **s})
+    evict = lambda **s: gae.paged_evict(**{**dict(k_pages=k, v_pages=k, page_table=table, seq_lens=ints, weights=w,  # noqa: E731
+                                                  dst_table=z(3, 1, dtype=torch.int32), keep=8), **s})
+    keys = lambda **s: gae.attention_key_weights(**{**dict(q=z(1, 2, 8, 64), k=z(1, 2, 8, 64), lse=z(1, 2, 8)), **s})  # noqa: E731
+    calls = [
+        lambda: append(k_new=new.float()), lambda: append(v_new=new[:, :, :3]), lambda: append(k_new=new[0]),
+        lambda: append(start=ints.long()), lambda: append(counts=ints[:2]), lambda: append(page_table=table.long()),
+        lambda: append(page_table=table[:2]), lambda: append(v_pages=k[:3]), lambda: append(k_pages=k.transpose(2, 3)),
+        lambda: append(k_new=z(3, 3, 5, 64, dtype=torch.bfloat16), v_new=z(3, 3, 5, 64, dtype=torch.bfloat16)),
+        lambda: attend(q=q[0]), lambda: attend(q=q.float()), lambda: attend(q=q[..., :32]),
+        lambda: attend(seq_lens=ints[:1]), lambda: attend(weights=w[..., :31]), lambda: attend(weights_out=w),
+        lambda: attend(weights=w.double()), lambda: attend(lse=z(3, 3)), lambda: attend(out=q.float()),
+        lambda: attend(page_table=table.t()),
+        lambda: evict(weights=w[:, :1]), lambda: evict(dst_table=z(2, 1, dtype=torch.int32)),
+        lambda: evict(seq_lens=ints.float()),
+        lambda: keys(q=z(2, 8, 64)), lambda: keys(k=z(1, 2, 8, 32)), lambda: keys(lse=z(1, 2, 7)),
+        lambda: keys(accumulate=True), lambda: keys(out=z(1, 2, 7)),
+        # all in order but for the device
+        append, attend, evict, keys,
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(gae.GAEError):
+            call()
+            pytest.fail(f"call {i} was accepted")
