@@ -24,6 +24,7 @@
 #include "crate_f32.cuh"
 #include "kv_cache.cuh"
 #include "key_weights.cuh"
+#include "paged_attn.cuh"
 
 namespace {
 

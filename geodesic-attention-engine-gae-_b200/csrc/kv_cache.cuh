@@ -14,12 +14,33 @@
 
 namespace gae {
 
+// Division of positions (< 2^31) by a run-time constant: q = (umulhi(n, mul) +
+// n) >> shift with shift = ceil(log2 d), mul = floor(2^32 (2^shift - d) / d) + 1
+// (T. Granlund, P. Montgomery, "Division by Invariant Integers using
+// Multiplication", 1994).  n < 2^31 keeps the sum within 32 bits.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    static FastDiv of(uint32_t d) {
+        uint32_t s = 0;
+        while ((1ull << s) < d) ++s;
+        return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+    }
+    __host__ __device__ __forceinline__ uint32_t div(uint32_t n) const {
+#ifdef __CUDA_ARCH__
+        return (__umulhi(n, mul) + n) >> shift;
+#else
+        return (uint32_t)((((uint64_t)n * mul) >> 32) + n) >> shift;
+#endif
+    }
+};
+
 // K and V pools [num_pages, kv_heads, page_size, head_dim], element strides.
 struct KvPool {
     void *k, *v;
     int64_t k_sp, k_sh, k_ss, v_sp, v_sh, v_ss;
     int64_t num_pages;
     int Hkv, page, D;
+    FastDiv by_page;
 };
 
 struct PageTable {
@@ -72,103 +93,6 @@ __global__ void paged_append_kernel(const AppendParams p) {
                                         (pg * p.pool.v_sp + h * p.pool.v_sh + slot * p.pool.v_ss) * ESIZE);
     kd[c] = __ldg(ks + c);
     vd[c] = __ldg(vs + c);
-}
-
-// ------------------------------------------------- single-token attention
-struct PagedAttnParams {
-    KvPool pool;
-    PageTable table;
-    const void *q;
-    void *o;
-    int64_t q_sb, q_sh, o_sb, o_sh;
-    const int *lens;
-    float *lse;           // [B, H], may be NULL
-    float *scores;        // [B, H, cap], with weights only
-    const float *w_in;    // [B, Hkv, >= len], with weights only
-    float *w_out;
-    int64_t wi_sb, wi_sh, wo_sb, wo_sh;
-    int B, H, cap;        // cap = max_pages * page_size
-    float scale_log2;
-};
-
-// One CTA per (head, sequence), one warp per key, lanes across head_dim.
-template <typename T>
-__global__ void __launch_bounds__(128) paged_attn_kernel(const PagedAttnParams p) {
-    constexpr int kPer = 8;  // head_dim <= 256
-    const int h = blockIdx.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int hk = h / (p.H / p.pool.Hkv), D = p.pool.D;
-    const int len = clamp_len(p.lens[b], p.cap);
-    float q[kPer], acc[kPer], m = -INFINITY, l = 0.f;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const int d = lane + 32 * j;
-        q[j] = d < D ? to_f<T>(static_cast<const T *>(p.q)[b * p.q_sb + h * p.q_sh + d]) : 0.f;
-        acc[j] = 0.f;
-    }
-    for (int pos = warp; pos < len; pos += 4) {
-        const int pg = page_of(p.table, p.pool.num_pages, b, pos / p.pool.page);
-        float *sc = p.scores ? p.scores + ((int64_t)b * p.H + h) * p.cap + pos : nullptr;
-        if (pg < 0) {
-            if (sc && lane == 0) *sc = -INFINITY;
-            continue;
-        }
-        const int slot = pos % p.pool.page;
-        const T *k = static_cast<const T *>(p.pool.k) + pg * p.pool.k_sp + hk * p.pool.k_sh + slot * p.pool.k_ss;
-        const T *v = static_cast<const T *>(p.pool.v) + pg * p.pool.v_sp + hk * p.pool.v_sh + slot * p.pool.v_ss;
-        float s = 0.f;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int d = lane + 32 * j;
-            if (d < D) s = fmaf(q[j], to_f<T>(k[d]), s);
-        }
-        for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-        s *= p.scale_log2;
-        if (sc && lane == 0) *sc = s;
-        // A row of -inf scores only has no weight anywhere; a NaN score reaches l and the output.
-        const float mn = fmaxf(m, s), base = mn == -INFINITY ? 0.f : mn;
-        const float a = exp2f(m - base), w = exp2f(s - base);
-        m = mn;
-        l = l * a + w;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int d = lane + 32 * j;
-            acc[j] = acc[j] * a + (d < D ? w * to_f<T>(v[d]) : 0.f);
-        }
-    }
-    __shared__ float sm[4], sl[4], so[4][256];
-    if (lane == 0) sm[warp] = m, sl[warp] = l;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) so[warp][lane + 32 * j] = acc[j];
-    __syncthreads();
-    m = fmaxf(fmaxf(sm[0], sm[1]), fmaxf(sm[2], sm[3]));
-    float f[4];
-    l = 0.f;
-    for (int w = 0; w < 4; ++w) {
-        f[w] = exp2f(sm[w] - (m == -INFINITY ? 0.f : m));
-        l += f[w] * sl[w];
-    }
-    for (int d = threadIdx.x; d < D; d += 128) {
-        float o = 0.f;
-        for (int w = 0; w < 4; ++w) o += f[w] * so[w][d];
-        static_cast<T *>(p.o)[b * p.o_sb + h * p.o_sh + d] = from_f<T>(l == 0.f ? 0.f : o / l);
-    }
-    if (threadIdx.x == 0 && p.lse)
-        p.lse[(int64_t)b * p.H + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * 0.6931471805599453f;
-}
-
-// w_out = w_in + sum over the group's heads of exp(score - lse), in head order.
-__global__ void paged_weights_kernel(const PagedAttnParams p) {
-    const int hk = blockIdx.y, b = blockIdx.z, pos = blockIdx.x * blockDim.x + threadIdx.x;
-    if (pos >= clamp_len(p.lens[b], p.cap)) return;
-    if (page_of(p.table, p.pool.num_pages, b, pos / p.pool.page) < 0) return;
-    const int G = p.H / p.pool.Hkv;
-    float w = 0.f;
-    for (int g = 0; g < G; ++g) {
-        const int64_t row = (int64_t)b * p.H + hk * G + g;
-        const float l = p.lse[row] * 1.4426950408889634f;
-        if (l != -INFINITY) w += exp2f(p.scores[row * p.cap + pos] - l);
-    }
-    p.w_out[b * p.wo_sb + hk * p.wo_sh + pos] = p.w_in[b * p.wi_sb + hk * p.wi_sh + pos] + w;
 }
 
 // ---------------------------------------------------------------- eviction

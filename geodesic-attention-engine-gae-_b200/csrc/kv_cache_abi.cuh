@@ -38,6 +38,7 @@ gae_status check_pool(const gae_kv_pool *pl, gae::KvPool *out) {
     out->v_sp = pl->v_stride[0]; out->v_sh = pl->v_stride[1]; out->v_ss = pl->v_stride[2];
     out->num_pages = pl->num_pages;
     out->Hkv = (int)pl->kv_heads; out->page = (int)pl->page_size; out->D = (int)pl->head_dim;
+    out->by_page = gae::FastDiv::of((uint32_t)pl->page_size);
     return GAE_OK;
 }
 
@@ -49,6 +50,78 @@ gae_status check_table(const int32_t *entry, int64_t stride, int64_t max_pages, 
         return fail(GAE_ERR_UNSUPPORTED, "a page table of more than 2^30 positions");
     out->entry = entry; out->stride = stride; out->max_pages = (int)max_pages;
     return GAE_OK;
+}
+
+// Workspace of one paged attention call (bytes, each region 256-byte aligned).
+struct PagedWs {
+    size_t parts, lse2, ml, o, scores, total;
+};
+PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool weights) {
+    const size_t blocks = (size_t)num_sms() * 2, heads = H / Hkv <= 8 ? 8 : 16;  // most of either, any type
+    PagedWs w;
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t was = at;
+        at += (n + 255) & ~(size_t)255;
+        return was;
+    };
+    w.parts = take((size_t)B * H * sizeof(int2));
+    w.lse2 = take((size_t)B * H * 4);
+    w.ml = take(blocks * 2 * heads * 2 * 4);
+    w.o = take(blocks * 2 * heads * D * 4);
+    w.scores = take(weights ? (size_t)B * H * cap * 4 : 0);
+    w.total = at;
+    return w;
+}
+
+// A launch that may begin while the one before it ends (it waits for it by griddepcontrol.wait).
+template <typename... Params, typename... Args>
+gae_status launch_after(void (*kern)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
+    cudaLaunchConfig_t c;
+    memset(&c, 0, sizeof(c));
+    c.gridDim = grid;
+    c.blockDim = dim3((unsigned)threads);
+    c.stream = st;
+    cudaLaunchAttribute at;
+    memset(&at, 0, sizeof(at));
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    GAE_CUDA_TRY(cudaLaunchKernelEx(&c, kern, args...));
+    return GAE_OK;
+}
+
+template <class Tile, int DM>
+gae_status launch_paged_attn(gae::PagedAttnParams p, cudaStream_t st) {
+    using Cfg = gae::PaCfg<Tile, DM>;
+    using T = typename Tile::Elem;
+    gae_status s;
+    if ((s = set_smem(gae::paged_attn_kernel<Tile, DM>, Cfg::kSmem)) != GAE_OK) return s;
+    p.groups = (p.G + Tile::kHeads - 1) / Tile::kHeads;
+    const int64_t rows = (int64_t)p.B * p.pool.Hkv * p.groups;
+    const int tile_keys = gae::kPaWarps * Tile::kKeys;
+    const int64_t most = rows * gae::max64(1, (p.cap + tile_keys - 1) / tile_keys);
+    const unsigned blocks = (unsigned)gae::min64(most, (int64_t)num_sms() * Cfg::kPerSm);
+    gae::paged_attn_kernel<Tile, DM><<<blocks, gae::kPaWarps * 32, Cfg::kSmem, st>>>(p);
+    GAE_CUDA_TRY(cudaGetLastError());
+    // A row of one tile is never split.
+    if (p.cap <= tile_keys && !p.scores) return GAE_OK;
+    const int64_t chunks = p.scores ? gae::min64((p.cap + gae::kJoinKeys - 1) / gae::kJoinKeys, 32768) : 0;
+    return launch_after(gae::paged_attn_join_kernel<T>, dim3((unsigned)rows, (unsigned)(Tile::kHeads + chunks)),
+                        gae::kJoinThreads, st, p, (int)Tile::kHeads);
+}
+
+template <int DM>
+gae_status launch_paged_attn_d(const gae::PagedAttnParams &p, gae_dtype t, cudaStream_t st) {
+    const bool few = p.G <= 8;
+    if (t == GAE_DTYPE_F32)
+        return p.G <= 2 ? launch_paged_attn<gae::PaFmaTile<DM, 2>, DM>(p, st) : launch_paged_attn<gae::PaFmaTile<DM, 8>, DM>(p, st);
+    if (t == GAE_DTYPE_BF16)
+        return few ? launch_paged_attn<gae::PaMmaTile<__nv_bfloat16, DM, 1>, DM>(p, st)
+                   : launch_paged_attn<gae::PaMmaTile<__nv_bfloat16, DM, 2>, DM>(p, st);
+    return few ? launch_paged_attn<gae::PaMmaTile<__half, DM, 1>, DM>(p, st)
+               : launch_paged_attn<gae::PaMmaTile<__half, DM, 2>, DM>(p, st);
 }
 
 }  // namespace
@@ -91,10 +164,9 @@ gae_status gae_paged_append(const gae_kv_pool *pool, const gae_paged_append_args
 size_t gae_paged_attn_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim,
                                       int64_t capacity, int with_weights) {
     if (batch < 1 || heads < 1 || kv_heads < 1 || head_dim < 1 || capacity < 0 || batch > 65535 || heads > 65535 ||
-        capacity > kMaxPositions)
+        capacity > kMaxPositions || heads % kv_heads || head_dim > 256 || batch * heads > INT32_MAX)
         return 0;
-    if (!with_weights) return 0;
-    return (size_t)batch * heads * (capacity + 1) * 4;
+    return paged_ws(batch, heads, kv_heads, head_dim, capacity, with_weights != 0).total;
 }
 
 gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args *a, void *stream) {
@@ -108,7 +180,8 @@ gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args
     if ((s = check_table(a->page_table, a->table_stride, a->max_pages, a->batch, pool->page_size, &p.table)) != GAE_OK)
         return s;
     if (a->batch == 0) return GAE_OK;
-    if (a->batch > 65535 || a->heads > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch or heads > 65535");
+    if (a->batch > 65535 || a->heads > 65535 || a->batch * a->heads > INT32_MAX)
+        return fail(GAE_ERR_UNSUPPORTED, "batch or heads > 65535, or more than 2^31 - 1 rows");
     const int es = dtype_size(pool->dtype);
     if (!a->q || !a->o || !a->seq_lens) return fail(GAE_ERR_INVALID_ARG, "NULL pointer in paged attention arguments");
     if (!aligned16(a->q) || !aligned16(a->o) || !row_strides(a->q_stride, 2, es) || !row_strides(a->o_stride, 2, es))
@@ -124,35 +197,32 @@ gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args
                     (long long)cap);
     const size_t need =
         gae_paged_attn_workspace_bytes(a->batch, a->heads, pool->kv_heads, pool->head_dim, cap, a->weights_out != nullptr);
-    if (need && (!a->workspace || !aligned16(a->workspace)))
+    if (!a->workspace || !aligned16(a->workspace))
         return fail(GAE_ERR_INVALID_ARG, "workspace is NULL or not 16-byte aligned");
     if (a->workspace_bytes < need)
         return fail(GAE_ERR_INVALID_ARG, "workspace too small: %zu < %zu", a->workspace_bytes, need);
     p.q = a->q; p.o = a->o; p.lse = a->lse; p.lens = a->seq_lens;
     p.q_sb = a->q_stride[0]; p.q_sh = a->q_stride[1]; p.o_sb = a->o_stride[0]; p.o_sh = a->o_stride[1];
     p.B = (int)a->batch; p.H = (int)a->heads; p.cap = (int)cap;
+    p.G = p.H / p.pool.Hkv;
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    const PagedWs w = paged_ws(a->batch, a->heads, pool->kv_heads, pool->head_dim, cap, a->weights_out != nullptr);
+    char *ws = static_cast<char *>(a->workspace);
+    p.parts = reinterpret_cast<int2 *>(ws + w.parts);
+    p.lse2 = reinterpret_cast<float *>(ws + w.lse2);
+    p.part_ml = reinterpret_cast<float *>(ws + w.ml);
+    p.part_o = reinterpret_cast<float *>(ws + w.o);
     if (a->weights_out) {
-        p.scores = static_cast<float *>(a->workspace);
-        if (!p.lse) p.lse = p.scores + (size_t)a->batch * a->heads * cap;
+        p.scores = reinterpret_cast<float *>(ws + w.scores);
         p.w_in = a->weights; p.w_out = a->weights_out;
         p.wi_sb = a->w_stride[0]; p.wi_sh = a->w_stride[1];
         p.wo_sb = a->w_out_stride[0]; p.wo_sh = a->w_out_stride[1];
     }
-    const dim3 grid((unsigned)a->heads, (unsigned)a->batch);
-    switch (pool->dtype) {
-        case GAE_DTYPE_F32: gae::paged_attn_kernel<float><<<grid, 128, 0, st>>>(p); break;
-        case GAE_DTYPE_BF16: gae::paged_attn_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(p); break;
-        case GAE_DTYPE_F16: gae::paged_attn_kernel<__half><<<grid, 128, 0, st>>>(p); break;
-    }
-    GAE_CUDA_TRY(cudaGetLastError());
-    if (a->weights_out && cap > 0) {
-        const dim3 g2((unsigned)((cap + 255) / 256), (unsigned)pool->kv_heads, (unsigned)a->batch);
-        gae::paged_weights_kernel<<<g2, 256, 0, st>>>(p);
-        GAE_CUDA_TRY(cudaGetLastError());
-    }
-    return GAE_OK;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    // Narrower heads than the tile's are padded with zeros in shared memory only.
+    if (pool->head_dim <= 64) return launch_paged_attn_d<64>(p, pool->dtype, st);
+    if (pool->head_dim <= 128) return launch_paged_attn_d<128>(p, pool->dtype, st);
+    return launch_paged_attn_d<256>(p, pool->dtype, st);
 }
 
 size_t gae_key_weights_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv) {
