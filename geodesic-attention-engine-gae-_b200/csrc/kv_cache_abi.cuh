@@ -57,7 +57,7 @@ struct PagedWs {
     size_t parts, lse2, ml, o, scores, total;
 };
 PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool weights) {
-    const size_t blocks = (size_t)num_sms() * 2, heads = H / Hkv <= 8 ? 8 : 16;  // most of either, any type
+    const size_t blocks = (size_t)num_sms() * 3, heads = H / Hkv <= 8 ? 8 : 16;  // most of either, any type
     PagedWs w;
     size_t at = 0;
     auto take = [&](size_t n) {

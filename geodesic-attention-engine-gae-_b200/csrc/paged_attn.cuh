@@ -46,12 +46,18 @@ struct PagedAttnParams {
     float *part_o;        // [blocks][2][heads of a tile][D]
 };
 
+#ifndef GAE_PA_STAGES
+#define GAE_PA_STAGES 2
+#endif
 constexpr int kPaWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool pred) {
     // src-size 0 writes zeros and reads nothing
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(pred ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -99,6 +105,7 @@ struct PaMmaTile {
     static constexpr int kHeads = NT * 8, kKeys = 16, kChunks = DM * 2 / 16;
     static constexpr int kWarpScratch = 0;
     using Elem = T;
+    __device__ explicit PaMmaTile(const float *) {}
     uint32_t qf[NT][DM / 16][2];
     float o[NT][DM / 16][4], m[NT][2], l[NT][2];
 
@@ -106,7 +113,7 @@ struct PaMmaTile {
     // rows of one chunk: the swizzle puts them in different banks).
     static __device__ __forceinline__ uint32_t at(int r, int c) { return r * (DM * 2) + ((c ^ (r & 7)) << 4); }
 
-    __device__ __forceinline__ void begin(const T *q, int64_t q_sh, int heads, int D, int lane, float *) {
+    __device__ __forceinline__ void load_q(const T *q, int64_t q_sh, int heads, int D, int lane) {
 #pragma unroll
         for (int n = 0; n < NT; ++n) {
             const int h = n * 8 + (lane >> 2);
@@ -118,6 +125,12 @@ struct PaMmaTile {
                     qf[n][kk][e] =
                         (h < heads && d < D) ? __ldg(reinterpret_cast<const unsigned *>(q + h * q_sh + d)) : 0u;
                 }
+        }
+    }
+
+    __device__ __forceinline__ void reset() {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) m[n][e] = -INFINITY, l[n][e] = 0.f;
 #pragma unroll
@@ -239,12 +252,14 @@ struct PaFmaTile {
     using Elem = float;
     const float *q;  // [HG][DM] in shared memory
     float o[HG][kVec], m[HG], l[HG];
+    __device__ explicit PaFmaTile(const float *q_smem) : q(q_smem) {}
 
     // Eight lanes (two rows, four chunks) read 128 bytes at a time.
     static __device__ __forceinline__ uint32_t at(int r, int c) { return r * (DM * 4) + ((c ^ ((r & 1) << 2)) << 4); }
 
-    __device__ __forceinline__ void begin(const float *, int64_t, int, int, int, float *q_smem) {
-        q = q_smem;
+    __device__ __forceinline__ void load_q(const float *, int64_t, int, int, int) {}
+
+    __device__ __forceinline__ void reset() {
 #pragma unroll
         for (int g = 0; g < HG; ++g) {
             m[g] = -INFINITY;
@@ -350,7 +365,7 @@ struct PaFmaTile {
 template <class Tile, int DM>
 struct PaCfg {
     static constexpr int kSlot = Tile::kKeys * DM * (int)sizeof(typename Tile::Elem) * 2;  // K and V rows of a warp
-    static constexpr int kStages = DM == 64 ? 6 : 3;
+    static constexpr int kStages = DM == 64 ? 2 * GAE_PA_STAGES : GAE_PA_STAGES;
     static constexpr int kRing = kPaWarps * kStages * kSlot;
     static constexpr int kOffMl = kRing;                                   // [warps][heads][2]
     static constexpr int kOffQ = kOffMl + kPaWarps * Tile::kHeads * 8;     // fp32 tiles: q [heads][DM]
@@ -359,7 +374,7 @@ struct PaCfg {
     static constexpr int kOffValid = kOffP + kPaWarps * Tile::kWarpScratch * 4;
     static constexpr int kOffScan = kOffValid + kPaWarps * kStages * 4;
     static constexpr int kSmem = (kOffScan + 64 + 15) / 16 * 16;
-    static constexpr int kPerSm = 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;
+    static constexpr int kPerSm = 3 * (kSmem + 1024) <= 228 * 1024 ? 3 : 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;
     // the merge reuses a stage: fp32 [heads][DM]
     static_assert(Tile::kHeads * DM * 4 <= kSlot, "a warp's O has to fit its stage");
     static_assert(kSmem <= 227 * 1024, "shared memory budget");
@@ -371,7 +386,7 @@ struct PaCursor {
 };
 
 template <class Tile, int DM>
-__global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     using Cfg = PaCfg<Tile, DM>;
     using T = typename Tile::Elem;
     constexpr int kKeys = Tile::kKeys, kTileKeys = kPaWarps * kKeys, kThreads = kPaWarps * 32;
@@ -429,118 +444,199 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
     ld.tiles = tiles_of(ld.len);
     cp = ld;
     int64_t row_begin = begin - cp.tile;  // first tile of the current row, in the total
-    auto advance = [&](PaCursor &c) {
-        if (++c.tile < c.tiles) return;
-        c.tile = 0;
-        if (++c.r < R) return;
-        c.r = 0;
-        if (++c.b >= p.B) return;
-        c.len = clamp_len(__ldg(p.lens + c.b), p.cap);
-        c.tiles = tiles_of(c.len);
-    };
 
-    // --- loader: each lane below kKeys looks its row's page up one tile ahead
+    // --- loader: pages are looked up one tile ahead of their copies
     const uint32_t ring = smem_u32(smem_pa) + warp * (Cfg::kStages * Cfg::kSlot);
     uint32_t *valid = reinterpret_cast<uint32_t *>(smem_pa + Cfg::kOffValid) + warp * Cfg::kStages;
-    int next_page = -1, next_slot = 0;
-    auto look_up = [&](const PaCursor &c) {
-        const int pos = c.tile * kTileKeys + warp * kKeys + (lane & (kKeys - 1));
+    constexpr int kRowChunks = Tile::kChunks, kPasses = kKeys * kRowChunks / 32, kElems = 16 / (int)sizeof(T);
+    constexpr int kRowsPerPass = 32 / kRowChunks > 0 ? 32 / kRowChunks : 1;
+    const int live_chunks = p.pool.D / kElems;
+    // Where a page holds whole warp tiles (its size a multiple of kKeys), the
+    // rows of a tile share one page and lie at one stride; full rows of such a
+    // tile need no predicate.
+    const bool one_page = p.pool.page % kKeys == 0;
+    const bool full_rows = live_chunks == kRowChunks;
+    const int *ld_table = p.table.entry + ld.b * p.table.stride;
+    const T *ld_k, *ld_v;
+    auto ld_head = [&] {
+        const int hk = ld.r / p.groups;
+        ld_k = static_cast<const T *>(p.pool.k) + hk * p.pool.k_sh;
+        ld_v = static_cast<const T *>(p.pool.v) + hk * p.pool.v_sh;
+    };
+    ld_head();
+    int next_page = -1, next_slot = 0, next_rows = 0;
+    auto look_up = [&] {  // the tile at ld
+        const int pos0 = ld.tile * kTileKeys + warp * kKeys;
+        const int pos = one_page ? pos0 : pos0 + (lane & (kKeys - 1));
         next_page = -1;
-        if (c.b < p.B && pos < c.len) {
+        next_rows = min(kKeys, ld.len - pos0);
+        if (pos < ld.len) {
             const uint32_t idx = p.pool.by_page.div(pos);
             next_slot = pos - (int)idx * p.pool.page;
-            next_page = page_of(p.table, p.pool.num_pages, c.b, (int)idx);
+            next_page = __ldg(ld_table + idx);
+            if ((int64_t)next_page >= p.pool.num_pages) next_page = -1;
         }
     };
-    constexpr int kRowChunks = Tile::kChunks, kPasses = kKeys * kRowChunks / 32;
-    const int live_chunks = p.pool.D * (int)sizeof(T) / 16;
-    auto load = [&](int stage) {  // the rows that look_up found, of head ld.r
-        const int hk = ld.r / p.groups;
-        const T *kb = static_cast<const T *>(p.pool.k) + hk * p.pool.k_sh;
-        const T *vb = static_cast<const T *>(p.pool.v) + hk * p.pool.v_sh;
-        const uint32_t mask = __ballot_sync(0xffffffffu, next_page >= 0 && lane < kKeys);
-        if (lane == 0) valid[stage] = mask;
-        if (mask != 0) {
-            const uint32_t sk = ring + stage * Cfg::kSlot, sv = sk + Cfg::kSlot / 2;
-#pragma unroll
-            for (int i = 0; i < kPasses; ++i) {
-                const int row = (i * 32 + lane) / kRowChunks, c = (i * 32 + lane) % kRowChunks;
-                const int pg = __shfl_sync(0xffffffffu, next_page, row), sl = __shfl_sync(0xffffffffu, next_slot, row);
-                const bool live = pg >= 0 && c < live_chunks;
-                const T *ks = kb, *vs = vb;
-                if (live) {
-                    ks += pg * p.pool.k_sp + sl * p.pool.k_ss + c * (16 / (int)sizeof(T));
-                    vs += pg * p.pool.v_sp + sl * p.pool.v_ss + c * (16 / (int)sizeof(T));
+    auto ld_advance = [&] {
+        if (++ld.tile >= ld.tiles) {
+            ld.tile = 0;
+            if (++ld.r >= R) {
+                ld.r = 0;
+                ++ld.b;  // another tile is issued only where there is another sequence
+                ld.len = 0;
+                if (ld.b < p.B) {
+                    ld.len = clamp_len(__ldg(p.lens + ld.b), p.cap);
+                    ld.tiles = tiles_of(ld.len);
+                    ld_table = p.table.entry + ld.b * p.table.stride;
                 }
-                cp_async16(sk + Tile::at(row, c), ks, live);
-                cp_async16(sv + Tile::at(row, c), vs, live);
             }
+            ld_head();
+        }
+        look_up();
+    };
+    auto load = [&](int stage) {  // the rows that look_up found
+        const uint32_t sk = ring + stage * Cfg::kSlot, sv = sk + Cfg::kSlot / 2;
+        if (one_page) {
+            const int rows = next_page >= 0 ? max(next_rows, 0) : 0;
+            if (lane == 0) valid[stage] = (1u << rows) - 1u;
+            if (rows == 0) return;
+            const int row0 = lane / kRowChunks, c = lane % kRowChunks;
+            const T *ks = ld_k + next_page * p.pool.k_sp + (next_slot + row0) * p.pool.k_ss + c * kElems;
+            const T *vs = ld_v + next_page * p.pool.v_sp + (next_slot + row0) * p.pool.v_ss + c * kElems;
+            if constexpr (kRowChunks <= 32) {
+                const int64_t kst = kRowsPerPass * p.pool.k_ss, vst = kRowsPerPass * p.pool.v_ss;
+                if (rows == kKeys && full_rows) {
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                        cp_async16(sk + Tile::at(row0 + i * kRowsPerPass, c), ks);
+                        cp_async16(sv + Tile::at(row0 + i * kRowsPerPass, c), vs);
+                        ks += kst;
+                        vs += vst;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < kPasses; ++i) {
+                        const bool live = row0 + i * kRowsPerPass < rows && c < live_chunks;
+                        cp_async16(sk + Tile::at(row0 + i * kRowsPerPass, c), live ? ks + i * kst : ld_k, live);
+                        cp_async16(sv + Tile::at(row0 + i * kRowsPerPass, c), live ? vs + i * vst : ld_v, live);
+                    }
+                }
+                return;
+            }
+        }
+        const int page_r = one_page ? (lane < next_rows ? next_page : -1) : next_page;
+        const int slot_r = one_page ? next_slot + (lane & (kKeys - 1)) : next_slot;
+        const uint32_t mask = __ballot_sync(0xffffffffu, page_r >= 0 && lane < kKeys);
+        if (lane == 0) valid[stage] = mask;
+        if (mask == 0) return;
+#pragma unroll
+        for (int i = 0; i < kPasses; ++i) {
+            const int row = (i * 32 + lane) / kRowChunks, c = (i * 32 + lane) % kRowChunks;
+            const int pg = __shfl_sync(0xffffffffu, page_r, row), sl = __shfl_sync(0xffffffffu, slot_r, row);
+            const bool live = pg >= 0 && c < live_chunks;
+            const T *ks = ld_k, *vs = ld_v;
+            if (live) {
+                ks += pg * p.pool.k_sp + sl * p.pool.k_ss + c * kElems;
+                vs += pg * p.pool.v_sp + sl * p.pool.v_ss + c * kElems;
+            }
+            cp_async16(sk + Tile::at(row, c), ks, live);
+            cp_async16(sv + Tile::at(row, c), vs, live);
         }
     };
 
     const int n_tiles = (int)(end - begin);
     int issued = 0;
-    look_up(ld);
+    look_up();
 #pragma unroll
     for (int s = 0; s < Cfg::kStages - 1; ++s) {
         if (issued < n_tiles) {
             load(s);
             ++issued;
-            advance(ld);
-            look_up(ld);
+            ld_advance();
         }
         cp_async_commit();
     }
 
-    Tile tile;
     float *q_smem = reinterpret_cast<float *>(smem_pa + Cfg::kOffQ);
+    Tile tile(q_smem);
     float *sp = reinterpret_cast<float *>(smem_pa + Cfg::kOffP) + warp * Tile::kWarpScratch;
-    bool fresh = true;
-    int stage = 0;
     int64_t row_start_tile = begin;  // where this block's part of the row starts
-    for (int it = 0; it < n_tiles; ++it) {
-        const int hk = cp.r / p.groups, h0 = (cp.r % p.groups) * Tile::kHeads;
-        const int heads = min(Tile::kHeads, p.G - h0);
-        const T *q = static_cast<const T *>(p.q) + cp.b * p.q_sb + (int64_t)(hk * p.G + h0) * p.q_sh;
-        if (fresh) {
-            if constexpr (Cfg::kQ) {
-                for (int i = tid; i < Tile::kHeads * DM; i += kThreads) {
-                    const int h = i / DM, d = i % DM;
-                    q_smem[i] = (h < heads && d < p.pool.D) ? q[h * p.q_sh + d] : 0.f;
-                }
-                __syncthreads();
-            }
-            tile.begin(q, p.q_sh, heads, p.pool.D, lane, q_smem);
-            fresh = false;
+    // The row at cp: its key head, first query head, their number, q and scores.
+    struct Row {
+        int b, r, hk, h0, heads;
+        const T *q;
+        float *scores;
+    } row;
+    auto set_row = [&] {
+        row.b = cp.b;
+        row.r = cp.r;
+        row.hk = cp.r / p.groups;
+        row.h0 = (cp.r % p.groups) * Tile::kHeads;
+        row.heads = min(Tile::kHeads, p.G - row.h0);
+        row.q = static_cast<const T *>(p.q) + cp.b * p.q_sb + (int64_t)(row.hk * p.G + row.h0) * p.q_sh;
+        row.scores =
+            p.scores ? p.scores + ((int64_t)cp.b * p.pool.Hkv + row.hk) * p.cap * p.G + row.h0 : nullptr;
+        tile.load_q(row.q, p.q_sh, row.heads, p.pool.D, lane);
+    };
+    auto stage_q = [&] {  // the fp32 tiles' q
+        if (!Cfg::kQ) return;
+        for (int i = tid; i < Tile::kHeads * DM; i += kThreads) {
+            const int h = i / DM, d = i % DM;
+            q_smem[i] = (h < row.heads && d < p.pool.D) ? to_f<T>(row.q[h * p.q_sh + d]) : 0.f;
         }
+    };
+    set_row();
+    stage_q();
+    tile.reset();
+    if constexpr (Cfg::kQ) __syncthreads();
+    int stage = 0;
+    for (int it = 0; it < n_tiles; ++it) {
         cp_async_wait<Cfg::kStages - 2>();
         __syncwarp();
+        // The stage before this one was read in the last turn: it is filled
+        // first, so that all stages but this are on their way meanwhile.
+        if (issued < n_tiles) {
+            load(stage == 0 ? Cfg::kStages - 1 : stage - 1);
+            ++issued;
+            ld_advance();
+        }
+        cp_async_commit();
         const uint32_t sk = ring + stage * Cfg::kSlot;
         const uint32_t mask = valid[stage];
         if (mask != 0) {
-            float *sc = nullptr;
-            if (p.scores)
-                sc = p.scores +
-                     (((int64_t)cp.b * p.pool.Hkv + hk) * p.cap + cp.tile * kTileKeys + warp * kKeys) * p.G + h0;
-            tile.step(sk, sk + Cfg::kSlot / 2, mask, p.scale_log2, lane, sc, p.G, heads, sp);
+            float *sc = row.scores ? row.scores + (int64_t)(cp.tile * kTileKeys + warp * kKeys) * p.G : nullptr;
+            tile.step(sk, sk + Cfg::kSlot / 2, mask, p.scale_log2, lane, sc, p.G, row.heads, sp);
         }
         __syncwarp();
-        const bool last = cp.tile + 1 == cp.tiles, stop = last || it + 1 == n_tiles;
-        if (stop) {
-            // --- the row's end here: the four warps' parts become one
+        const bool last = cp.tile + 1 == cp.tiles;
+        if (last || it + 1 == n_tiles) {
+            // --- the row's end here: the four warps' parts become one.  The next
+            // row's q is on its way meanwhile.
+            const Row done = row;
+            const int row_tiles = cp.tiles;
+            cp.tile = -1;
+            if (it + 1 < n_tiles) {
+                if (++cp.r == R) {
+                    cp.r = 0;
+                    ++cp.b;
+                    cp.len = clamp_len(__ldg(p.lens + cp.b), p.cap);
+                    cp.tiles = tiles_of(cp.len);
+                }
+                set_row();
+            }
             float *so = reinterpret_cast<float *>(smem_pa + warp * (Cfg::kStages * Cfg::kSlot) + stage * Cfg::kSlot);
             float *sml = reinterpret_cast<float *>(smem_pa + Cfg::kOffMl);
             tile.finish(so, sml + warp * Tile::kHeads * 2, lane);
             __syncthreads();
+            if (it + 1 < n_tiles) stage_q();
             const bool first = row_start_tile == row_begin, whole = first && last;
-            const int row = cp.b * R + cp.r;
             const int part = blockIdx.x * 2 + (first ? 1 : 0);
             if (first && tid == 0) {
                 // the block that holds tile t of the total is floor(((t + 1) * blocks - 1) / total)
-                const int64_t t = row_begin + cp.tiles - 1;
-                p.parts[row] = make_int2((int)blockIdx.x, (int)(((t + 1) * blocks - 1) / total));
+                const int64_t t = row_begin + row_tiles - 1;
+                p.parts[done.b * R + done.r] = make_int2((int)blockIdx.x, (int)(((t + 1) * blocks - 1) / total));
             }
-            for (int i = tid; i < heads * (DM / 4); i += kThreads) {
+            for (int i = tid; i < done.heads * (DM / 4); i += kThreads) {
                 const int h = i / (DM / 4), d = i % (DM / 4) * 4;
                 float mw[kPaWarps], mx = -INFINITY, l = 0.f;
 #pragma unroll
@@ -562,7 +658,7 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
                 if (d >= p.pool.D) continue;
                 if (whole) {
                     const float inv = l == 0.f ? 0.f : 1.f / l;
-                    T *o = static_cast<T *>(p.o) + cp.b * p.o_sb + (int64_t)(hk * p.G + h0 + h) * p.o_sh + d;
+                    T *o = static_cast<T *>(p.o) + done.b * p.o_sb + (int64_t)(done.hk * p.G + done.h0 + h) * p.o_sh + d;
                     if constexpr (sizeof(T) == 4) {
                         *reinterpret_cast<float4 *>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
                     } else {
@@ -571,7 +667,7 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
                     }
                     if (d == 0) {
                         const float l2 = l == 0.f ? -INFINITY : base + log2f(l);
-                        const int64_t hh = (int64_t)cp.b * p.H + hk * p.G + h0 + h;
+                        const int64_t hh = (int64_t)done.b * p.H + done.hk * p.G + done.h0 + h;
                         p.lse2[hh] = l2;
                         if (p.lse) p.lse[hh] = l2 * kLn2;
                     }
@@ -582,18 +678,11 @@ __global__ void __launch_bounds__(kPaWarps * 32) paged_attn_kernel(const __grid_
                 }
             }
             __syncthreads();  // the stage may be loaded again
-            fresh = true;
-            row_begin += cp.tiles;
+            tile.reset();
+            row_begin += row_tiles;
             row_start_tile = row_begin;
         }
-        if (issued < n_tiles) {
-            load(stage == 0 ? Cfg::kStages - 1 : stage - 1);
-            ++issued;
-            advance(ld);
-            look_up(ld);
-        }
-        cp_async_commit();
-        advance(cp);
+        ++cp.tile;
         stage = stage + 1 == Cfg::kStages ? 0 : stage + 1;
     }
     cp_async_wait<0>();

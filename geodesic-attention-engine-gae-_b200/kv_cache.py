@@ -19,8 +19,9 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+import struct
 
-from . import GAEError, _check, _dtype_code, _torch, lib
+from . import GAEError, _check, _torch, lib
 
 _I64_2, _I64_3 = C.c_int64 * 2, C.c_int64 * 3
 
@@ -70,6 +71,19 @@ class PagedEvictArgs(C.Structure):
                 ("new_lens", C.c_void_p), ("kept", C.c_void_p), ("kept_weights", C.c_void_p)]
 
 
+def _packer(mirror):
+    """struct packer of a mirror's fields in their C layout: one call fills a
+    whole argument block, in a fifth of the time a ctypes structure takes."""
+    code = {C.c_void_p: "P", C.c_int64: "q", C.c_size_t: "N", C.c_int: "i", C.c_float: "f", _I64_2: "2q", _I64_3: "3q"}
+    s = struct.Struct("@" + "".join(code[t] for _, t in mirror._fields_) + "0q")
+    assert s.size == C.sizeof(mirror)
+    return s.pack
+
+
+_pack_pool, _pack_append, _pack_attn, _pack_keys, _pack_evict = map(
+    _packer, (KvPool, PagedAppendArgs, PagedAttnArgs, KeyWeightsArgs, PagedEvictArgs))
+
+
 def _bind(L):
     vp, i64, sz = C.c_void_p, C.c_int64, C.c_size_t
     for name in ("gae_paged_append", "gae_paged_attn_fwd", "gae_paged_evict"):
@@ -81,63 +95,87 @@ def _bind(L):
     L.gae_key_weights.argtypes = [vp, vp]
 
 
-def _run(device, stream, tensors, body):
+def _run(what, tensors, stream, body):
     """body(stream pointer) with the tensors' device and `stream` current, so that
     what it allocates belongs to the stream it runs on; on a stream other than
-    the current one the inputs are marked as used there."""
+    the current one the inputs are marked as used there.  tensors: by name, the
+    first one's device is everyone's."""
     torch = _torch()
-    if stream is None and torch.cuda.current_device() == device.index:
-        return body(torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.device(device):
+    dev = -2
+    for name, t in tensors:
+        if t is not None:
+            i = t.get_device()
+            if dev == -2:
+                dev = i
+            if i != dev or i < 0:
+                raise GAEError(1, f"{what}: tensors must be on one CUDA device, {name} is on {t.device}")
+    if stream is None and torch.cuda.current_device() == dev:
+        return body(torch._C._cuda_getCurrentRawStream(dev))
+    with torch.cuda.device(dev):
         if stream is None:
-            return body(torch.cuda.current_stream().cuda_stream)
-        if stream.device != device:
-            raise GAEError(1, f"stream on {stream.device}, tensors on {device}")
+            return body(torch._C._cuda_getCurrentRawStream(dev))
+        if stream.device.index != dev:
+            raise GAEError(1, f"{what}: stream on {stream.device}, tensors on device {dev}")
         with torch.cuda.stream(stream):
-            for t in tensors:
+            for _, t in tensors:
                 if t is not None:
                     t.record_stream(stream)
             return body(stream.cuda_stream)
 
 
-def _same_device(what, device, **tensors):
-    if device.type != "cuda":
-        raise GAEError(1, f"{what}: tensors must be on a CUDA device")
-    for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise GAEError(1, f"{what}: {name} is on {t.device}, not {device}")
+_CODES = None
+
+
+def _code(t):
+    global _CODES
+    if _CODES is None:
+        torch = _torch()
+        _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+    c = _CODES.get(t.dtype)
+    if c is None:
+        raise GAEError(1, f"unsupported dtype {t.dtype}")
+    return c
 
 
 def _pool(what, k_pages, v_pages):
-    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+    """(packed gae_kv_pool, shape)"""
+    shape = k_pages.shape
+    if len(shape) != 4 or v_pages.shape != shape:
         raise GAEError(1, f"{what}: k_pages and v_pages must be [num_pages, kv_heads, page_size, head_dim]")
     if v_pages.dtype != k_pages.dtype:
         raise GAEError(1, f"{what}: k_pages and v_pages must share a dtype")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    kp, kh, ks, kd = k_pages.stride()
+    vp, vh, vs, vd = v_pages.stride()
+    if kd != 1 or vd != 1:
         raise GAEError(1, f"{what}: pages must have a contiguous head_dim")
-    return KvPool(k_pages.data_ptr(), v_pages.data_ptr(), _I64_3(*ks[:3]), _I64_3(*vs[:3]), *k_pages.shape,
-                  _dtype_code(k_pages))
+    return _pack_pool(k_pages.data_ptr(), v_pages.data_ptr(), kp, kh, ks, vp, vh, vs, *shape, _code(k_pages)), shape
 
 
 def _table(what, table, batch, name="page_table"):
-    if table.dim() != 2 or table.shape[0] != batch or table.dtype != _torch().int32 or \
-            (table.shape[1] > 1 and table.stride(1) != 1):
-        raise GAEError(1, f"{what}: {name} must be int32 [batch, max_pages] with contiguous rows")
-    return table.data_ptr(), table.stride(0), table.shape[1]
+    shape = table.shape
+    if len(shape) != 2 or shape[0] != batch or table.dtype != _torch().int32:
+        raise GAEError(1, f"{what}: {name} must be int32 [batch, max_pages]")
+    row, one = table.stride()
+    if one != 1 and shape[1] > 1:
+        raise GAEError(1, f"{what}: {name} must have contiguous rows")
+    return table.data_ptr(), row, shape[1]
 
 
 def _ints(what, t, batch, name):
-    if t.dim() != 1 or t.shape[0] != batch or t.dtype != _torch().int32 or not t.is_contiguous():
+    if t.dtype != _torch().int32 or t.shape != (batch,) or not t.is_contiguous():
         raise GAEError(1, f"{what}: {name} must be contiguous int32 [batch]")
     return t.data_ptr()
 
 
 def _weights(what, t, batch, heads, n, name):
-    if t.dim() != 3 or t.shape[0] != batch or t.shape[1] != heads or t.shape[2] < n or \
-            t.dtype != _torch().float32 or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise GAEError(1, f"{what}: {name} must be fp32 [{batch}, {heads}, >= {n}] with contiguous rows")
-    return t.data_ptr(), _I64_2(t.stride(0), t.stride(1))
+    """(address, batch stride, head stride)"""
+    shape = t.shape
+    if len(shape) != 3 or shape[0] != batch or shape[1] != heads or shape[2] < n or t.dtype != _torch().float32:
+        raise GAEError(1, f"{what}: {name} must be fp32 [{batch}, {heads}, >= {n}]")
+    sb, sh, one = t.stride()
+    if one != 1 and shape[2] > 1:
+        raise GAEError(1, f"{what}: {name} must have contiguous rows")
+    return t.data_ptr(), sb, sh
 
 
 def paged_append(k_new, v_new, k_pages, v_pages, page_table, start, *, counts=None, stream=None):
@@ -146,24 +184,25 @@ def paged_append(k_new, v_new, k_pages, v_pages, page_table, start, *, counts=No
     becomes position start[b] + t.  Tokens beyond the page table, or whose entry
     names no page, are dropped."""
     what = "paged_append"
-    if k_new.dim() != 4 or v_new.shape != k_new.shape:
+    shape = k_new.shape
+    if len(shape) != 4 or v_new.shape != shape:
         raise GAEError(1, f"{what}: k_new and v_new must be [batch, kv_heads, tokens, head_dim]")
-    B, H, T, D = k_new.shape
-    if k_pages.dim() != 4 or k_pages.shape[1] != H or k_pages.shape[3] != D:
+    B, H, T, D = shape
+    pool, ps = _pool(what, k_pages, v_pages)
+    if ps[1] != H or ps[3] != D:
         raise GAEError(1, f"{what}: k_new and k_pages differ in heads or head_dim")
     if k_new.dtype != k_pages.dtype or v_new.dtype != k_pages.dtype:
         raise GAEError(1, f"{what}: new rows and pages must share a dtype")
-    pool = _pool(what, k_pages, v_pages)
-    ks, vs = k_new.stride(), v_new.stride()
-    if ks[3] != 1 or vs[3] != 1:
+    kb, kh, kt, kd = k_new.stride()
+    vb, vh, vt, vd = v_new.stride()
+    if kd != 1 or vd != 1:
         raise GAEError(1, f"{what}: new rows must have a contiguous head_dim")
-    a = PagedAppendArgs(k_new.data_ptr(), v_new.data_ptr(), _I64_3(*ks[:3]), _I64_3(*vs[:3]), B, T,
-                        *_table(what, page_table, B), _ints(what, start, B, "start"),
-                        None if counts is None else _ints(what, counts, B, "counts"))
-    _same_device(what, k_pages.device, v_pages=v_pages, k_new=k_new, v_new=v_new, page_table=page_table,
-                 start=start, counts=counts)
-    _run(k_pages.device, stream, (k_new, v_new, k_pages, v_pages, page_table, start, counts),
-         lambda st: _check(lib().gae_paged_append(C.byref(pool), C.byref(a), st)))
+    a = _pack_append(k_new.data_ptr(), v_new.data_ptr(), kb, kh, kt, vb, vh, vt, B, T,
+                     *_table(what, page_table, B), _ints(what, start, B, "start"),
+                     0 if counts is None else _ints(what, counts, B, "counts"))
+    _run(what, (("k_pages", k_pages), ("v_pages", v_pages), ("k_new", k_new), ("v_new", v_new),
+                ("page_table", page_table), ("start", start), ("counts", counts)), stream,
+         lambda st: _check(lib().gae_paged_append(pool, a, st)))
 
 
 def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, out=None, lse=None,
@@ -174,58 +213,55 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
     gives 0 and lse -inf.
 
     weights (fp32 [B, Hkv, >= the page table's positions]) asks for the keys'
-    attention weight: weights_out = weights + the softmax summed over each key head's
-    query heads; weights_out defaults to weights (in place).  Positions without
-    a key are left as they are."""
+    attention weight: weights_out = weights + the softmax summed over each key
+    head's query heads; weights_out defaults to weights (in place).  Positions
+    without a key are left as they are."""
     what = "paged_attention"
     torch = _torch()
-    if q.dim() != 3:
+    shape = q.shape
+    if len(shape) != 3:
         raise GAEError(1, f"{what}: q must be [batch, heads, head_dim]")
-    B, H, D = q.shape
-    pool = _pool(what, k_pages, v_pages)
-    if k_pages.shape[3] != D or k_pages.dtype != q.dtype:
+    B, H, D = shape
+    pool, (_, Hkv, page, pd) = _pool(what, k_pages, v_pages)
+    if pd != D or k_pages.dtype != q.dtype:
         raise GAEError(1, f"{what}: q and the pages differ in head_dim or dtype")
-    Hkv, page = k_pages.shape[1], k_pages.shape[2]
     table = _table(what, page_table, B)
     lens = _ints(what, seq_lens, B, "seq_lens")
-    if q.stride(2) != 1:
+    qb, qh, qd = q.stride()
+    if qd != 1:
         raise GAEError(1, f"{what}: q must have a contiguous head_dim")
-    if out is not None and (out.shape != q.shape or out.dtype != q.dtype or out.stride(2) != 1):
+    if out is not None and (out.shape != shape or out.dtype != q.dtype or out.stride(2) != 1):
         raise GAEError(1, f"{what}: out must be like q, with a contiguous head_dim")
     if lse is not None and (lse.shape != (B, H) or lse.dtype != torch.float32 or not lse.is_contiguous()):
         raise GAEError(1, f"{what}: lse must be contiguous fp32 [batch, heads]")
     cap = table[2] * page
-    w = wo = None
-    w_st = wo_st = _I64_2(0, 0)
-    w_len = 0
+    w = wo = (0, 0, 0)
     if weights is not None:
         weights_out = weights if weights_out is None else weights_out
-        w, w_st = _weights(what, weights, B, Hkv, cap, "weights")
-        wo, wo_st = _weights(what, weights_out, B, Hkv, cap, "weights_out")
-        w_len = cap
+        w = _weights(what, weights, B, Hkv, cap, "weights")
+        wo = _weights(what, weights_out, B, Hkv, cap, "weights_out")
     elif weights_out is not None:
         raise GAEError(1, f"{what}: weights_out without weights")
-    dev = k_pages.device
-    _same_device(what, dev, q=q, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, out=out, lse=lse,
-                 weights=weights, weights_out=weights_out)
     L = lib()
 
     def body(st):
         o, l = out, lse
         if o is None:
-            o = torch.empty((B, H, D), dtype=q.dtype, device=dev)
+            o = torch.empty_like(q)
         if return_lse and l is None:
-            l = torch.empty((B, H), dtype=torch.float32, device=dev)
-        n = L.gae_paged_attn_workspace_bytes(B, H, Hkv, D, cap, w is not None)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        a = PagedAttnArgs(q.data_ptr(), o.data_ptr(), None if l is None else l.data_ptr(),
-                          _I64_2(q.stride(0), q.stride(1)), _I64_2(o.stride(0), o.stride(1)), B, H, *table, lens,
-                          1.0 / math.sqrt(D) if scale is None else scale, w, wo, w_st, wo_st, w_len,
-                          ws.data_ptr() if n else None, n)
-        _check(L.gae_paged_attn_fwd(C.byref(pool), C.byref(a), st))
+            l = torch.empty((B, H), dtype=torch.float32, device=q.device)
+        n = L.gae_paged_attn_workspace_bytes(B, H, Hkv, D, cap, weights is not None)
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        ob, oh, _ = o.stride()
+        a = _pack_attn(q.data_ptr(), o.data_ptr(), 0 if l is None else l.data_ptr(), qb, qh, ob, oh, B, H, *table,
+                       lens, 1.0 / math.sqrt(D) if scale is None else scale, w[0], wo[0], *w[1:], *wo[1:], cap,
+                       ws.data_ptr(), n)
+        _check(L.gae_paged_attn_fwd(pool, a, st))
         return (o, l) if return_lse else o
 
-    return _run(dev, stream, (q, k_pages, v_pages, page_table, seq_lens, out, lse, weights, weights_out), body)
+    return _run(what, (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
+                       ("seq_lens", seq_lens), ("out", out), ("lse", lse), ("weights", weights),
+                       ("weights_out", weights_out)), stream, body)
 
 
 def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv_offset=0, out=None,
@@ -239,68 +275,69 @@ def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv
     view of a cache's weights; accumulate=True adds to it."""
     what = "attention_key_weights"
     torch = _torch()
-    if q.dim() != 4 or k.dim() != 4:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 4 or len(ks) != 4:
         raise GAEError(1, f"{what}: q and k must be [batch, heads, seq, head_dim]")
-    B, H, Nq, D = q.shape
-    Hkv, Nkv = k.shape[1], k.shape[2]
-    if k.shape[0] != B or k.shape[3] != D or k.dtype != q.dtype:
+    B, H, Nq, D = qs
+    Hkv, Nkv = ks[1], ks[2]
+    if ks[0] != B or ks[3] != D or k.dtype != q.dtype:
         raise GAEError(1, f"{what}: q and k differ in batch, head_dim or dtype")
-    if q.stride(3) != 1 or k.stride(3) != 1:
+    qb, qh, qn, qd = q.stride()
+    kb, kh, kn, kd = k.stride()
+    if qd != 1 or kd != 1:
         raise GAEError(1, f"{what}: q and k must have a contiguous head_dim")
-    if lse.shape != (B, H, Nq) or lse.dtype != torch.float32 or (Nq > 1 and lse.stride(2) != 1):
-        raise GAEError(1, f"{what}: lse must be fp32 [batch, heads, seq_q] with contiguous rows")
+    l = _weights(what, lse, B, H, Nq, "lse")
+    if lse.shape[2] != Nq:
+        raise GAEError(1, f"{what}: lse must be [batch, heads, seq_q]")
     if accumulate and out is None:
         raise GAEError(1, f"{what}: accumulate needs out")
     if out is not None and out.shape != (B, Hkv, Nkv):
         raise GAEError(1, f"{what}: out must be [{B}, {Hkv}, {Nkv}]")
-    dev = q.device
-    _same_device(what, dev, k=k, lse=lse, out=out)
     L = lib()
-    scale = 1.0 / math.sqrt(D) if scale is None else scale
 
     def body(st):
-        w = torch.empty((B, Hkv, Nkv), dtype=torch.float32, device=dev) if out is None else out
-        o, os_ = _weights(what, w, B, Hkv, Nkv, "out")
+        w = torch.empty((B, Hkv, Nkv), dtype=torch.float32, device=q.device) if out is None else out
         n = L.gae_key_weights_workspace_bytes(B, H, Hkv, Nq, Nkv)
-        ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-        a = KeyWeightsArgs(q.data_ptr(), k.data_ptr(), lse.data_ptr(), o, B, H, Hkv, Nq, Nkv, D,
-                           _I64_3(*q.stride()[:3]), _I64_3(*k.stride()[:3]),
-                           _I64_2(lse.stride(0), lse.stride(1)), os_, _dtype_code(q), 1 if causal else 0,
-                           1 if accumulate else 0, scale, q_offset, kv_offset, ws.data_ptr() if n else None, n)
-        _check(L.gae_key_weights(C.byref(a), st))
+        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        wp, wb, wh = _weights(what, w, B, Hkv, Nkv, "out")
+        a = _pack_keys(q.data_ptr(), k.data_ptr(), l[0], wp, B, H, Hkv, Nq, Nkv, D, qb, qh, qn, kb, kh, kn,
+                       *l[1:], wb, wh, _code(q), 1 if causal else 0, 1 if accumulate else 0,
+                       1.0 / math.sqrt(D) if scale is None else scale, q_offset, kv_offset,
+                       ws.data_ptr() if n else 0, n)
+        _check(L.gae_key_weights(a, st))
         return w
 
-    return _run(dev, stream, (q, k, lse, out), body)
+    return _run(what, (("q", q), ("k", k), ("lse", lse), ("out", out)), stream, body)
 
 
 def paged_evict(k_pages, v_pages, page_table, seq_lens, weights, dst_table, *, keep, recent=0, stream=None):
     """Brings every sequence to at most `keep` cached positions: per key head the
     `recent` last positions and those of the largest weights (fp32 [B, Hkv, n];
-    a sequence is cut to n; equal weights: the lower position, NaN largest).  The kept
-    rows are copied in order to positions 0, 1, ... of dst_table, whose pages
+    a sequence is cut to n; equal weights: the lower position, NaN largest).  The
+    kept rows are copied in order to positions 0, 1, ... of dst_table, whose pages
     must not be among those read.  Returns (new lengths int32 [B], kept
     positions int32 [B, Hkv, keep], -1 beyond the length, their weights fp32,
     0 beyond)."""
     what = "paged_evict"
     torch = _torch()
-    pool = _pool(what, k_pages, v_pages)
-    Hkv, B = k_pages.shape[1], page_table.shape[0]
+    pool, (_, Hkv, _, _) = _pool(what, k_pages, v_pages)
+    B = page_table.shape[0]
     table = _table(what, page_table, B)
     dst = _table(what, dst_table, B, "dst_table")
     lens = _ints(what, seq_lens, B, "seq_lens")
-    w, w_st = _weights(what, weights, B, Hkv, 0, "weights")
-    dev = k_pages.device
-    _same_device(what, dev, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, weights=weights,
-                 dst_table=dst_table)
-    keep, recent = int(keep), int(recent)
+    w = _weights(what, weights, B, Hkv, 0, "weights")
+    if keep < 1:
+        raise GAEError(1, f"{what}: keep must be positive")
 
     def body(st):
-        new_lens = torch.empty(B, dtype=torch.int32, device=dev)
-        kept = torch.empty((B, Hkv, max(keep, 0)), dtype=torch.int32, device=dev)
-        kept_w = torch.empty((B, Hkv, max(keep, 0)), dtype=torch.float32, device=dev)
-        a = PagedEvictArgs(B, *table, lens, w, w_st, weights.shape[2], *dst, keep, recent, new_lens.data_ptr(),
-                           kept.data_ptr(), kept_w.data_ptr())
-        _check(lib().gae_paged_evict(C.byref(pool), C.byref(a), st))
+        dev = k_pages.device
+        new_lens = torch.empty_like(seq_lens)
+        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+        kept_w = torch.empty((B, Hkv, keep), dtype=torch.float32, device=dev)
+        a = _pack_evict(B, *table, lens, *w, weights.shape[2], *dst, keep, recent, new_lens.data_ptr(),
+                        kept.data_ptr(), kept_w.data_ptr())
+        _check(lib().gae_paged_evict(pool, a, st))
         return new_lens, kept, kept_w
 
-    return _run(dev, stream, (k_pages, v_pages, page_table, seq_lens, weights, dst_table), body)
+    return _run(what, (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
+                       ("seq_lens", seq_lens), ("weights", weights), ("dst_table", dst_table)), stream, body)
