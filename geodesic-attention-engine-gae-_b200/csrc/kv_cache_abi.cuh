@@ -108,8 +108,9 @@ gae_status launch_paged_attn(gae::PagedAttnParams p, cudaStream_t st) {
     // A row of one tile is never split.
     if (p.cap <= tile_keys && !p.scores) return GAE_OK;
     const int64_t chunks = p.scores ? gae::min64((p.cap + gae::kJoinKeys - 1) / gae::kJoinKeys, 32768) : 0;
-    return launch_after(gae::paged_attn_join_kernel<T>, dim3((unsigned)rows, (unsigned)(Tile::kHeads + chunks)),
-                        gae::kJoinThreads, st, p, (int)Tile::kHeads);
+    const int heads = p.G < Tile::kHeads ? p.G : Tile::kHeads;
+    return launch_after(gae::paged_attn_join_kernel<T>, dim3((unsigned)rows, (unsigned)(heads + chunks)),
+                        gae::kJoinThreads, st, p, (int)Tile::kHeads, heads);
 }
 
 template <int DM>

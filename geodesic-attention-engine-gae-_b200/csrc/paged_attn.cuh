@@ -250,9 +250,10 @@ struct PaFmaTile {
     static constexpr int kWarpScratch = kKeys * HG;  // probabilities, floats
     static constexpr int kVec = DM / 32;             // columns of a lane
     using Elem = float;
-    const float *q;  // [HG][DM] in shared memory
-    float o[HG][kVec], m[HG], l[HG];
-    __device__ explicit PaFmaTile(const float *q_smem) : q(q_smem) {}
+    uint32_t q;  // [HG][DM] in shared memory
+    uint64_t o[HG][kVec / 2];  // pairs of columns
+    float m[HG], l[HG];
+    __device__ explicit PaFmaTile(const float *q_smem) : q(smem_u32(q_smem)) {}
 
     // Eight lanes (two rows, four chunks) read 128 bytes at a time.
     static __device__ __forceinline__ uint32_t at(int r, int c) { return r * (DM * 4) + ((c ^ ((r & 1) << 2)) << 4); }
@@ -265,31 +266,40 @@ struct PaFmaTile {
             m[g] = -INFINITY;
             l[g] = 0.f;
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) o[g][j] = 0.f;
+            for (int j = 0; j < kVec / 2; ++j) o[g][j] = 0;
         }
     }
 
-    static __device__ __forceinline__ float4 lds4(uint32_t a) {
-        float4 v;
-        asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-        return v;
+    // 16 bytes as two pairs for the packed arithmetic
+    static __device__ __forceinline__ void lds_pairs(uint32_t a, uint64_t &lo, uint64_t &hi) {
+        asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(lo), "=l"(hi) : "r"(a) : "memory");
+    }
+    static __device__ __forceinline__ float sum2(uint64_t v) {
+        float a, b;
+        f2_unpack(v, a, b);
+        return a + b;
     }
 
     __device__ __forceinline__ void step(uint32_t sk, uint32_t sv, uint32_t valid, float scale_log2, int lane,
                                          float *scores, int G, int heads, float *sp) {
         const int r = lane >> 2, quarter = lane & 3;
-        float s[HG] = {};
+        float s[HG];
+        {
+            uint64_t acc[HG] = {};
 #pragma unroll
-        for (int i = 0; i < DM / 16; ++i) {
-            const float4 kv = lds4(sk + at(r, i * 4 + quarter));
+            for (int i = 0; i < DM / 16; ++i) {
+                uint64_t k0, k1;
+                lds_pairs(sk + at(r, i * 4 + quarter), k0, k1);
 #pragma unroll
-            for (int g = 0; g < HG; ++g) {
-                const float4 qv = *reinterpret_cast<const float4 *>(q + g * DM + (i * 4 + quarter) * 4);
-                s[g] = fmaf(kv.x, qv.x, s[g]);
-                s[g] = fmaf(kv.y, qv.y, s[g]);
-                s[g] = fmaf(kv.z, qv.z, s[g]);
-                s[g] = fmaf(kv.w, qv.w, s[g]);
+                for (int g = 0; g < HG; ++g) {
+                    uint64_t q0, q1;
+                    lds_pairs(q + (g * DM + (i * 4 + quarter) * 4) * 4, q0, q1);
+                    acc[g] = f2_fma(k0, q0, acc[g]);
+                    acc[g] = f2_fma(k1, q1, acc[g]);
+                }
             }
+#pragma unroll
+            for (int g = 0; g < HG; ++g) s[g] = sum2(acc[g]);
         }
         const bool ok = ((valid >> r) & 1u) != 0;
         bool grow = false;
@@ -312,7 +322,7 @@ struct PaFmaTile {
                 m[g] = mx;
                 l[g] *= alpha;
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) o[g][j] *= alpha;
+                for (int j = 0; j < kVec / 2; ++j) o[g][j] = f2_mul(o[g][j], f2_pack(alpha, alpha));
             }
         }
 #pragma unroll
@@ -324,23 +334,20 @@ struct PaFmaTile {
         __syncwarp();
 #pragma unroll
         for (int k = 0; k < kKeys; ++k) {
-            float v[kVec], p[HG];
-#pragma unroll
-            for (int g = 0; g < HG; ++g) p[g] = sp[k * HG + g];
+            uint64_t v[kVec / 2];
             if constexpr (kVec == 2) {
-                const uint32_t a = sv + at(k, lane >> 1) + (lane & 1) * 8;
-                asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "r"(a) : "memory");
+                asm volatile("ld.shared.b64 %0, [%1];" : "=l"(v[0]) : "r"(sv + at(k, lane >> 1) + (lane & 1) * 8) : "memory");
             } else {
 #pragma unroll
-                for (int j = 0; j < kVec / 4; ++j) {
-                    const float4 t = lds4(sv + at(k, j * 32 + lane));
-                    v[4 * j] = t.x, v[4 * j + 1] = t.y, v[4 * j + 2] = t.z, v[4 * j + 3] = t.w;
-                }
+                for (int j = 0; j < kVec / 4; ++j) lds_pairs(sv + at(k, j * 32 + lane), v[2 * j], v[2 * j + 1]);
             }
 #pragma unroll
-            for (int g = 0; g < HG; ++g)
+            for (int g = 0; g < HG; ++g) {
+                const float pg = sp[k * HG + g];
+                const uint64_t p2 = f2_pack(pg, pg);
 #pragma unroll
-                for (int j = 0; j < kVec; ++j) o[g][j] = fmaf(p[g], v[j], o[g][j]);
+                for (int j = 0; j < kVec / 2; ++j) o[g][j] = f2_fma(p2, v[j], o[g][j]);
+            }
         }
         __syncwarp();  // sp is rewritten by the next step
     }
@@ -354,9 +361,9 @@ struct PaFmaTile {
             t += __shfl_xor_sync(0xffffffffu, t, 16);
             if (lane == 0) ml[2 * g] = m[g], ml[2 * g + 1] = t;
 #pragma unroll
-            for (int j = 0; j < kVec; ++j) {
-                const int d = kVec == 2 ? lane * 2 + j : (j >> 2) * 128 + lane * 4 + (j & 3);
-                so[g * DM + (d ^ (((g >> 1) & 3) << 3))] = o[g][j];
+            for (int j = 0; j < kVec / 2; ++j) {
+                const int d = kVec == 2 ? lane * 2 : (j >> 1) * 128 + lane * 4 + (j & 1) * 2;
+                *reinterpret_cast<uint64_t *>(so + g * DM + (d ^ (((g >> 1) & 3) << 3))) = o[g][j];
             }
         }
     }
@@ -500,39 +507,39 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
             const int rows = next_page >= 0 ? max(next_rows, 0) : 0;
             if (lane == 0) valid[stage] = (1u << rows) - 1u;
             if (rows == 0) return;
-            const int row0 = lane / kRowChunks, c = lane % kRowChunks;
-            const T *ks = ld_k + next_page * p.pool.k_sp + (next_slot + row0) * p.pool.k_ss + c * kElems;
-            const T *vs = ld_v + next_page * p.pool.v_sp + (next_slot + row0) * p.pool.v_ss + c * kElems;
-            if constexpr (kRowChunks <= 32) {
-                const int64_t kst = kRowsPerPass * p.pool.k_ss, vst = kRowsPerPass * p.pool.v_ss;
-                if (rows == kKeys && full_rows) {
+            // Pass i: row row0 + i * kRowsPerPass, or half a row where it has 64 pieces.
+            constexpr int kHalves = kRowChunks > 32 ? kRowChunks / 32 : 1;
+            const int row0 = lane / kRowChunks, c0 = lane % kRowChunks;
+            const T *ks = ld_k + next_page * p.pool.k_sp + (next_slot + row0) * p.pool.k_ss + c0 * kElems;
+            const T *vs = ld_v + next_page * p.pool.v_sp + (next_slot + row0) * p.pool.v_ss + c0 * kElems;
+            const int64_t kst = kRowsPerPass * p.pool.k_ss, vst = kRowsPerPass * p.pool.v_ss;
+            if (rows == kKeys && full_rows) {
 #pragma unroll
-                    for (int i = 0; i < kPasses; ++i) {
-                        cp_async16(sk + Tile::at(row0 + i * kRowsPerPass, c), ks);
-                        cp_async16(sv + Tile::at(row0 + i * kRowsPerPass, c), vs);
-                        ks += kst;
-                        vs += vst;
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kPasses; ++i) {
-                        const bool live = row0 + i * kRowsPerPass < rows && c < live_chunks;
-                        cp_async16(sk + Tile::at(row0 + i * kRowsPerPass, c), live ? ks + i * kst : ld_k, live);
-                        cp_async16(sv + Tile::at(row0 + i * kRowsPerPass, c), live ? vs + i * vst : ld_v, live);
-                    }
+                for (int i = 0; i < kPasses; ++i) {
+                    const int r = row0 + i / kHalves * kRowsPerPass, half = i % kHalves * 32;
+                    cp_async16(sk + Tile::at(r, c0 + half), ks + half * kElems);
+                    cp_async16(sv + Tile::at(r, c0 + half), vs + half * kElems);
+                    if (i % kHalves == kHalves - 1) ks += kst, vs += vst;
                 }
-                return;
+            } else {
+#pragma unroll
+                for (int i = 0; i < kPasses; ++i) {
+                    const int r = row0 + i / kHalves * kRowsPerPass, half = i % kHalves * 32;
+                    const bool live = r < rows && c0 + half < live_chunks;
+                    cp_async16(sk + Tile::at(r, c0 + half), live ? ks + half * kElems : ld_k, live);
+                    cp_async16(sv + Tile::at(r, c0 + half), live ? vs + half * kElems : ld_v, live);
+                    if (i % kHalves == kHalves - 1) ks += kst, vs += vst;
+                }
             }
+            return;
         }
-        const int page_r = one_page ? (lane < next_rows ? next_page : -1) : next_page;
-        const int slot_r = one_page ? next_slot + (lane & (kKeys - 1)) : next_slot;
-        const uint32_t mask = __ballot_sync(0xffffffffu, page_r >= 0 && lane < kKeys);
+        const uint32_t mask = __ballot_sync(0xffffffffu, next_page >= 0 && lane < kKeys);
         if (lane == 0) valid[stage] = mask;
         if (mask == 0) return;
 #pragma unroll
         for (int i = 0; i < kPasses; ++i) {
             const int row = (i * 32 + lane) / kRowChunks, c = (i * 32 + lane) % kRowChunks;
-            const int pg = __shfl_sync(0xffffffffu, page_r, row), sl = __shfl_sync(0xffffffffu, slot_r, row);
+            const int pg = __shfl_sync(0xffffffffu, next_page, row), sl = __shfl_sync(0xffffffffu, next_slot, row);
             const bool live = pg >= 0 && c < live_chunks;
             const T *ks = ld_k, *vs = ld_v;
             if (live) {
@@ -689,117 +696,129 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
 }
 
 // Joins the parts of rows that more than one block worked on: block (row, y), y
-// < heads of a tile, joins head y; further blocks of the row's key head add up
-// the keys' weights, 1024 positions at a time.
+// < join_heads, joins head y; further blocks of the row's key head add up
+// the keys' weights, kJoinKeys positions at a time.  The kernel is all latency:
+// every thread reads its parts' statistics and sums side by side and scales as
+// it goes, so that one trip to memory follows the row's entry in `parts`.
 constexpr int kJoinThreads = 256, kJoinKeys = 1024;
 
+// (m, l) and (m2, l2), sums relative to 2^m, become one; f and f2 scale what
+// was summed beside them.
+__device__ __forceinline__ void join_sums(float &m, float &l, float m2, float l2, float &f, float &f2) {
+    const float mx = fmaxf(m, m2), base = mx == -INFINITY ? 0.f : mx;
+    f = ex2_approx(m - base);
+    f2 = ex2_approx(m2 - base);
+    l = f * l + f2 * l2;
+    m = mx;
+}
+
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p, int tile_heads) {
+__global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p, int tile_heads, int join_heads) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int R = p.pool.Hkv * p.groups, row = blockIdx.x, b = row / R, r = row % R, D = p.pool.D;
     const int hk = r / p.groups, tid = threadIdx.x;
-    // (maximum, sum) of head h of row `rw` over its parts, by the whole block
-    __shared__ float red[2][kJoinThreads / 32];
-    auto part_at = [&](int2 ps, int i, int h) {
-        const int blk = ps.x + i;
-        return ((int64_t)blk * 2 + (i == 0 ? 1 : 0)) * tile_heads + h;  // the first block's part starts the row
+    auto part_at = [&](int2 ps, int i, int h) {  // the first block's part starts the row
+        return ((int64_t)(ps.x + i) * 2 + (i == 0 ? 1 : 0)) * tile_heads + h;
     };
-    auto join_stats = [&](int2 ps, int h, float &mx, float &l) {
-        const int n = ps.y - ps.x + 1;
-        mx = -INFINITY;
-        for (int i = tid; i < n; i += kJoinThreads) mx = fmaxf(mx, p.part_ml[part_at(ps, i, h) * 2]);
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-        __syncthreads();
-        if ((tid & 31) == 0) red[0][tid >> 5] = mx;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < kJoinThreads / 32; ++w) mx = fmaxf(mx, red[0][w]);
-        const float base = mx == -INFINITY ? 0.f : mx;
-        l = 0.f;
-        for (int i = tid; i < n; i += kJoinThreads) {
-            const int64_t at = part_at(ps, i, h) * 2;
-            l += ex2_approx(p.part_ml[at] - base) * p.part_ml[at + 1];
-        }
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if ((tid & 31) == 0) red[1][tid >> 5] = l;
-        __syncthreads();
-        l = 0.f;
-#pragma unroll
-        for (int w = 0; w < kJoinThreads / 32; ++w) l += red[1][w];
-        mx = base;
-    };
-    if ((int)blockIdx.y < tile_heads) {
+    const float2 *ml = reinterpret_cast<const float2 *>(p.part_ml);
+    if ((int)blockIdx.y < join_heads) {
         const int h = blockIdx.y, h0 = (r % p.groups) * tile_heads;
         if (h0 + h >= p.G) return;
         const int2 ps = p.parts[row];
         if (ps.x == ps.y) return;
-        float base, l;
-        join_stats(ps, h, base, l);
         // float4 columns across threads, parts across what is left of them
         __shared__ float4 sum[kJoinThreads];
-        const int cols = D / 4, lanes = kJoinThreads / cols, c = tid % cols, part0 = tid / cols;
+        __shared__ float2 stat[kJoinThreads];
+        const int cols = D / 4, lanes = kJoinThreads / cols, c = tid % cols, lane0 = tid / cols;
+        const int n = ps.y - ps.x + 1;
         float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (part0 < lanes) {
-            const int n = ps.y - ps.x + 1;
+        float m = -INFINITY, l = 0.f, f, f2;
+        if (lane0 < lanes)
 #pragma unroll 4
-            for (int i = part0; i < n; i += lanes) {
+            for (int i = lane0; i < n; i += lanes) {
                 const int64_t at = part_at(ps, i, h);
-                const float f = ex2_approx(p.part_ml[at * 2] - base);
+                const float2 s = ml[at];
                 const float4 x = *reinterpret_cast<const float4 *>(p.part_o + at * D + c * 4);
-                acc.x += f * x.x, acc.y += f * x.y, acc.z += f * x.z, acc.w += f * x.w;
+                join_sums(m, l, s.x, s.y, f, f2);
+                acc.x = f * acc.x + f2 * x.x, acc.y = f * acc.y + f2 * x.y;
+                acc.z = f * acc.z + f2 * x.z, acc.w = f * acc.w + f2 * x.w;
             }
-        }
         sum[tid] = acc;
+        if (c == 0 && lane0 < lanes) stat[lane0] = make_float2(m, l);
         __syncthreads();
         if (tid < cols) {
-            for (int i = 1; i < lanes; ++i) {
+            for (int i = 1; i < min(lanes, n); ++i) {
                 const float4 x = sum[i * cols + tid];
-                acc.x += x.x, acc.y += x.y, acc.z += x.z, acc.w += x.w;
+                join_sums(m, l, stat[i].x, stat[i].y, f, f2);
+                acc.x = f * acc.x + f2 * x.x, acc.y = f * acc.y + f2 * x.y;
+                acc.z = f * acc.z + f2 * x.z, acc.w = f * acc.w + f2 * x.w;
             }
             const float inv = l == 0.f ? 0.f : 1.f / l;
             T *o = static_cast<T *>(p.o) + b * p.o_sb + (int64_t)(hk * p.G + h0 + h) * p.o_sh + tid * 4;
             o[0] = from_f<T>(acc.x * inv), o[1] = from_f<T>(acc.y * inv);
             o[2] = from_f<T>(acc.z * inv), o[3] = from_f<T>(acc.w * inv);
             if (tid == 0 && p.lse)
-                p.lse[(int64_t)b * p.H + hk * p.G + h0 + h] = l == 0.f ? -INFINITY : (base + log2f(l)) * kLn2;
+                p.lse[(int64_t)b * p.H + hk * p.G + h0 + h] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
         return;
     }
     // weights: once per key head, by its first row's blocks
     if (r % p.groups) return;
     const int len = clamp_len(__ldg(p.lens + b), p.cap);
-    constexpr int kPer = kJoinKeys / kJoinThreads;
-    for (int first = ((int)blockIdx.y - tile_heads) * kJoinKeys; first < len;
-         first += ((int)gridDim.y - tile_heads) * kJoinKeys) {
-        float w[kPer] = {};
-        for (int grp = 0; grp < p.groups; ++grp) {
-            const int2 ps = p.parts[row + grp];
-            for (int h = 0; h < tile_heads && grp * tile_heads + h < p.G; ++h) {
-                const int g = grp * tile_heads + h;
+    int first = ((int)blockIdx.y - join_heads) * kJoinKeys;
+    if (first >= len) return;
+    constexpr int kPer = kJoinKeys / kJoinThreads, kWarps = kJoinThreads / 32;
+    __shared__ float lse2[kWarps * 2];
+    const int warp = tid >> 5, lane = tid & 31;
+    const float *scores = p.scores + ((int64_t)b * p.pool.Hkv + hk) * p.cap * p.G;
+    for (; first < len; first += ((int)gridDim.y - join_heads) * kJoinKeys) {
+        float was[kPer], w[kPer] = {};
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+            const int pos = first + i * kJoinThreads + tid;
+            was[i] = pos < len ? p.w_in[b * p.wi_sb + hk * p.wi_sh + pos] : 0.f;
+        }
+        for (int g0 = 0; g0 < p.G; g0 += kWarps * 2) {  // 16 heads' statistics at a time, two to a warp
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int g = g0 + warp + e * kWarps;
+                if (g >= p.G) break;
+                const int2 ps = p.parts[row + g / tile_heads];
                 float l2;
                 if (ps.x == ps.y) {
                     l2 = p.lse2[(int64_t)b * p.H + hk * p.G + g];
                 } else {
-                    float base, l;
-                    join_stats(ps, h, base, l);
-                    l2 = l == 0.f ? -INFINITY : base + log2f(l);
+                    float m = -INFINITY, l = 0.f, f, f2;
+                    for (int i = lane; i <= ps.y - ps.x; i += 32) {
+                        const float2 s = ml[part_at(ps, i, g % tile_heads)];
+                        join_sums(m, l, s.x, s.y, f, f2);
+                    }
+#pragma unroll
+                    for (int o = 16; o > 0; o >>= 1) {
+                        const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, l, o);
+                        join_sums(m, l, m2, s2, f, f2);
+                    }
+                    l2 = l == 0.f ? -INFINITY : m + log2f(l);
                 }
-                if (l2 == -INFINITY) continue;
+                // a row without a finite score has no weight to hand out
+                if (lane == 0) lse2[warp + e * kWarps] = l2 == -INFINITY ? INFINITY : l2;
+            }
+            __syncthreads();
+            const int many = min(p.G - g0, kWarps * 2);
+#pragma unroll 4
+            for (int g = 0; g < many; ++g)
 #pragma unroll
                 for (int i = 0; i < kPer; ++i) {
                     const int pos = first + i * kJoinThreads + tid;
-                    if (pos < len)
-                        w[i] += ex2_approx(p.scores[(((int64_t)b * p.pool.Hkv + hk) * p.cap + pos) * p.G + g] - l2);
+                    if (pos < len) w[i] += ex2_approx(scores[(int64_t)pos * p.G + g0 + g] - lse2[g]);
                 }
-            }
         }
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
             const int pos = first + i * kJoinThreads + tid;
             if (pos >= len || page_of(p.table, p.pool.num_pages, b, (int)p.pool.by_page.div(pos)) < 0) continue;
-            p.w_out[b * p.wo_sb + hk * p.wo_sh + pos] = p.w_in[b * p.wi_sb + hk * p.wi_sh + pos] + w[i];
+            p.w_out[b * p.wo_sb + hk * p.wo_sh + pos] = was[i] + w[i];
         }
     }
 }

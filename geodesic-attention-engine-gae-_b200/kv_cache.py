@@ -18,6 +18,7 @@ and may be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes as C
+import functools
 import math
 import struct
 
@@ -93,6 +94,11 @@ def _bind(L):
     L.gae_key_weights_workspace_bytes.restype = sz
     L.gae_key_weights_workspace_bytes.argtypes = [i64] * 5
     L.gae_key_weights.argtypes = [vp, vp]
+
+
+@functools.lru_cache(maxsize=1024)
+def _attn_workspace(*sizes):
+    return lib().gae_paged_attn_workspace_bytes(*sizes)
 
 
 def _run(what, tensors, stream, body):
@@ -250,7 +256,7 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
             o = torch.empty_like(q)
         if return_lse and l is None:
             l = torch.empty((B, H), dtype=torch.float32, device=q.device)
-        n = L.gae_paged_attn_workspace_bytes(B, H, Hkv, D, cap, weights is not None)
+        n = _attn_workspace(B, H, Hkv, D, cap, weights is not None)
         ws = torch.empty(n, dtype=torch.uint8, device=q.device)
         ob, oh, _ = o.stride()
         a = _pack_attn(q.data_ptr(), o.data_ptr(), 0 if l is None else l.data_ptr(), qb, qh, ob, oh, B, H, *table,
