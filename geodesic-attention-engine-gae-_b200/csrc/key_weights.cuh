@@ -1,84 +1,325 @@
 // key_weights.cuh -- the attention weight that a block of queries puts on each
-// key: w[b, hk, j] = sum over the heads h of key head hk and the queries i that
-// see key j of exp(scale <q_i, k_j> - lse_i), from the forward's log-sum-exp.
+// key, from the forward's log-sum-exp:
+//
+//   w[b, hk, j] = sum over the heads h of key head hk, sum over the queries i
+//                 that see key j of exp(scale <q_i, k_j> - lse_i)
+//
 // No reference counterpart; it is what an eviction after a prompt goes by.
+//
+// The scores are computed transposed, keys as the 128 rows of a tcgen05 tile
+// and queries as its columns: a TMEM lane is then one key, so a thread adds up
+// its key's weights in registers and no two threads ever share a sum (no
+// atomics, the same bits every time).  One CTA per (128-key tile, key head,
+// batch): K stays in shared memory, the tiles of 128 queries of all the head's
+// query heads stream through a TMA ring, two S tiles alternate in TMEM so that
+// the next product runs while eight warps exponentiate the last.  Two CTAs to
+// an SM.
+//
+// What bounds it: one exponential per score.  The MUFU gives 16 a cycle and
+// SM, a 128 x 128 tile takes it 1024 cycles where the products at head_dim 128
+// take 512; every kKwPolyPeriod-th pair therefore goes to a polynomial on the
+// FMA pipe.
 #pragma once
-#include "attn_f32.cuh"
+#include "attn_bwd_sm100.cuh"
 #include "sm100.cuh"
 
 namespace gae {
 
 struct KeyWeightsParams {
-    const void *q, *k;
+    CUtensorMap tm_q, tm_k;  // dims {D, N, H, B}, box {64 elements, 128 rows}, 128B swizzle
     const float *lse;
-    float *out;
-    int64_t q_sb, q_sh, q_ss, k_sb, k_sh, k_ss, l_sb, l_sh, o_sb, o_sh;
-    int B, H, Hkv, Nq, Nkv, D, causal, accumulate;
-    int64_t off;  // query row r sees key c iff c <= r + off (causal)
+    float *out;              // [B, Hkv, Nkv], or the splits' parts
+    int64_t l_sb, l_sh, o_sb, o_sh;
+    int64_t part;            // elements between two splits' parts; 0: one split, written to out
+    int B, H, Hkv, Nq, Nkv, causal, accumulate, splits;
+    int64_t off;             // query row r sees key c iff c <= r + off (causal)
     float scale_log2;
 };
 
-// One CTA per (64-key tile, key head, batch): 16 x 16 threads, each 4 keys x 4
-// queries of a 64 x 64 tile of scores, queries streamed.
-template <typename T>
-__global__ void __launch_bounds__(256) key_weights_kernel(const KeyWeightsParams p) {
-    extern __shared__ float smem_kw[];
-    float *sk = smem_kw, *sq = smem_kw + 64 * (p.D + 1);
-    __shared__ float slse[64], red[64][17];
-    const int hk = blockIdx.y, b = blockIdx.z, k0 = blockIdx.x * 64;
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;  // tx: queries, ty: keys
-    const int G = p.H / p.Hkv, ld = p.D + 1;
-    const T *kp = static_cast<const T *>(p.k) + b * p.k_sb + hk * p.k_sh;
-    for (int i = threadIdx.x; i < 64 * p.D; i += 256) {
-        const int r = i / p.D, d = i % p.D;
-        sk[r * ld + d] = k0 + r < p.Nkv ? to_f<T>(kp[(k0 + r) * p.k_ss + d]) : 0.f;
+enum KeyWeightsWaitSite : unsigned {
+    kSiteKwK = 0x501, kSiteKwQFull = 0x502, kSiteKwQEmpty = 0x503, kSiteKwS = 0x504, kSiteKwSEmpty = 0x505,
+    kSiteKwDone = 0x506, kSiteKwSmem = 0x507,
+};
+
+#ifndef GAE_KW_POLY_PERIOD
+#define GAE_KW_POLY_PERIOD 2
+#endif
+constexpr int kKwPolyPeriod = GAE_KW_POLY_PERIOD;
+
+// 2^x for a pair of x <= 2^22 on the FMA pipe: exp2_poly_x2's range reduction
+// with a polynomial of degree 5, whose coefficients are the minimax fit of 2^f
+// on [0, 1) in relative error (by linear programming over 4001 points; max
+// relative error 7.5e-8, 1.5e-7 in fp32), as exact as the MUFU's 2^-22.  Results
+// below 2^-126 come out as 2^-126.
+__device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
+    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
+    float x0, x1;
+    f2_unpack(x2, x0, x1);
+    const uint64_t xc = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
+    const uint64_t mg = f2_pack(kMagic, kMagic);
+    uint64_t t, j, f;
+    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(xc), "l"(mg));
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(j) : "l"(t), "l"(mg));
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(xc), "l"(j));
+    uint64_t p = f2_fma(f, f2_pack(0.00187757204f, 0.00187757204f), f2_pack(0.00898935273f, 0.00898935273f));
+    p = f2_fma(p, f, f2_pack(0.0558263063f, 0.0558263063f));
+    p = f2_fma(p, f, f2_pack(0.240153626f, 0.240153626f));
+    p = f2_fma(p, f, f2_pack(0.693153083f, 0.693153083f));
+    p = f2_fma(p, f, f2_pack(0.99999994f, 0.99999994f));
+    float p0, p1, t0, t1;
+    f2_unpack(p, p0, p1);
+    f2_unpack(t, t0, t1);
+    // bits(t) * 2^23 puts j into the exponent field; adding bits(p) scales p by 2^j
+    return f2_pack(__uint_as_float(__float_as_uint(t0) * 8388608u + __float_as_uint(p0)),
+                   __uint_as_float(__float_as_uint(t1) * 8388608u + __float_as_uint(p1)));
+}
+
+template <int D>
+struct KeyWeightsCfg {
+    static constexpr int kBox = 128 * 128, kPanels = D * 2 / 128, kTile = kPanels * kBox;
+    static constexpr int kStages = D == 128 ? 2 : 4;
+    static constexpr int kOffK = 0, kOffQ = kTile, kOffLse = kOffQ + kStages * kTile;  // lse: 4 tiles of 128
+    static constexpr int kOffRed = kOffLse + 4 * 128 * 4;                               // 128 sums of the upper columns
+    static constexpr int kOffBar = kOffRed + 128 * 4;
+    static constexpr int kNumBars = 2 + 2 * kStages + 4;  // k, done, q_full/q_empty, s_full/s_empty [2]
+    static constexpr int kPayload = kOffBar + kNumBars * 8 + 16;
+    static constexpr int kSmem = kPayload + 1024;  // slack for the 1024-byte alignment of the swizzle atoms
+    static constexpr int kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kLseWarp = 10, kThreads = 11 * 32;
+    static constexpr uint32_t kTmemCols = 256;
+    static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs to an SM");
+};
+
+template <int D, bool kBF16>
+__global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
+    key_weights_kernel(const __grid_constant__ KeyWeightsParams p) {
+    using Cfg = KeyWeightsCfg<D>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw_addr = smem_u32(smem_raw), base = (raw_addr + 1023u) & ~1023u;
+    uint8_t *smem = smem_raw + (base - raw_addr);
+    if (base - raw_addr + Cfg::kPayload > (uint32_t)Cfg::kSmem) {
+        if (threadIdx.x == 0) record_error(kSiteKwSmem);
+        return;
     }
-    float w[4] = {};
-    for (int g = 0; g < G; ++g) {
-        const int h = hk * G + g;
-        const T *qp = static_cast<const T *>(p.q) + b * p.q_sb + h * p.q_sh;
-        for (int q0 = 0; q0 < p.Nq; q0 += 64) {
-            if (p.causal && k0 > q0 + 63 + p.off) continue;
-            __syncthreads();
-            for (int i = threadIdx.x; i < 64 * p.D; i += 256) {
-                const int r = i / p.D, d = i % p.D;
-                sq[r * ld + d] = q0 + r < p.Nq ? to_f<T>(qp[(q0 + r) * p.q_ss + d]) : 0.f;
+    const uint32_t sK = base + Cfg::kOffK, sBar = base + Cfg::kOffBar;
+    auto sQ = [&](int st) { return base + Cfg::kOffQ + st * Cfg::kTile; };
+    float *s_lse = reinterpret_cast<float *>(smem + Cfg::kOffLse), *s_red = reinterpret_cast<float *>(smem + Cfg::kOffRed);
+    const uint32_t bar_k = sBar, bar_done = sBar + 8;
+    auto bar_q_full = [&](int st) { return sBar + 8u * (2 + st); };
+    auto bar_q_empty = [&](int st) { return sBar + 8u * (2 + Cfg::kStages + st); };
+    auto bar_s_full = [&](int bf) { return sBar + 8u * (2 + 2 * Cfg::kStages + bf); };
+    auto bar_s_empty = [&](int bf) { return sBar + 8u * (4 + 2 * Cfg::kStages + bf); };
+    uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::kOffBar + Cfg::kNumBars * 8);
+    volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
+    volatile int no_abort = 0;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    // Key tiles in ascending order: under a causal mask the first have the most queries.
+    const int rows = p.B * p.Hkv;
+    const int j = blockIdx.x / rows, b = blockIdx.x % rows / p.Hkv, hk = blockIdx.x % rows % p.Hkv, split = blockIdx.y;
+    const int G = p.H / p.Hkv, nq = (p.Nq + 127) / 128;
+    int i0 = 0;  // first query tile that sees a key of this tile
+    if (p.causal) i0 = (int)min64(nq, max64(0, (int64_t)j * 128 - p.off) / 128);
+    const int per_head = nq - i0, all = per_head * G;
+    const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
+    const int n_it = t1 - t0;
+    auto tile_of = [&](int it, int &h, int &q0) {  // query tile it of this CTA
+        const int t = t0 + it;
+        h = hk * G + t / per_head;
+        q0 = (i0 + t % per_head) * 128;
+    };
+
+    if (threadIdx.x == 0) {
+        mbar_init(bar_k, 1);
+        mbar_init(bar_done, 1);
+        for (int st = 0; st < Cfg::kStages; ++st) {
+            mbar_init(bar_q_full(st), 1);
+            mbar_init(bar_q_empty(st), 1);
+        }
+        for (int bf = 0; bf < 2; ++bf) {
+            mbar_init(bar_s_full(bf), 1 + 32);  // the products, and the lanes of the lse warp
+            mbar_init(bar_s_empty(bf), Cfg::kEpiWarps * 32);
+        }
+        *abort_flag = 0;
+        fence_mbar_init();
+    }
+    if (warp == Cfg::kMmaWarp) {
+        tmem_alloc(smem_u32(tmem_slot), Cfg::kTmemCols);
+        tmem_relinquish();
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *tmem_slot;
+
+    float total = 0.f;
+    if (warp == Cfg::kTmaWarp) {
+        if (lane == 0 && n_it > 0) {
+            tma_prefetch_desc(&p.tm_q);
+            mbar_expect_tx(bar_k, Cfg::kTile);
+            for (int hf = 0; hf < Cfg::kPanels; ++hf)
+                tma_load_4d(sK + hf * Cfg::kBox, &p.tm_k, bar_k, hf * 64, j * 128, hk, b);
+            int it = 0;
+            for (; it < n_it; ++it) {
+                const int st = it % Cfg::kStages, use = it / Cfg::kStages;
+                if (use > 0 && !mbar_wait(bar_q_empty(st), (use - 1) & 1, kSiteKwQEmpty, abort_flag)) break;
+                int h, q0;
+                tile_of(it, h, q0);
+                mbar_expect_tx(bar_q_full(st), Cfg::kTile);
+                for (int hf = 0; hf < Cfg::kPanels; ++hf)
+                    tma_load_4d(sQ(st) + hf * Cfg::kBox, &p.tm_q, bar_q_full(st), hf * 64, q0, h, b);
             }
-            if (threadIdx.x < 64) {
-                const int r = q0 + threadIdx.x;
-                const float l = r < p.Nq ? p.lse[b * p.l_sb + h * p.l_sh + r] : -INFINITY;
-                slse[threadIdx.x] = l == -INFINITY ? INFINITY : l * 1.4426950408889634f;  // such a row weighs nothing
-            }
-            __syncthreads();
-            float s[4][4] = {};
-            for (int d = 0; d < p.D; ++d) {
-                float a[4], c[4];
+            // the copies issued have landed before the CTA exits
+            mbar_wait(bar_k, 0, kSiteKwK, &no_abort);
+            for (int u = max(0, it - Cfg::kStages); u < it; ++u)
+                mbar_wait(bar_q_full(u % Cfg::kStages), (u / Cfg::kStages) & 1, kSiteKwQFull, &no_abort);
+        }
+    } else if (warp == Cfg::kMmaWarp) {
+        if (lane == 0 && n_it > 0) {
+            constexpr uint32_t id = idesc_f16(128, 128, kBF16, false, false);
+            bool ok = mbar_wait(bar_k, 0, kSiteKwK, abort_flag);
+            for (int it = 0; it < n_it && ok; ++it) {
+                const int st = it % Cfg::kStages, bf = it & 1;
+                if (it >= 2 && !(ok = mbar_wait(bar_s_empty(bf), ((it >> 1) - 1) & 1, kSiteKwSEmpty, abort_flag))) break;
+                if (!(ok = mbar_wait(bar_q_full(st), (it / Cfg::kStages) & 1, kSiteKwQFull, abort_flag))) break;
+                tc_fence_after();
 #pragma unroll
-                for (int e = 0; e < 4; ++e) a[e] = sk[(ty * 4 + e) * ld + d], c[e] = sq[(tx * 4 + e) * ld + d];
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-#pragma unroll
-                    for (int f = 0; f < 4; ++f) s[e][f] = fmaf(a[e], c[f], s[e][f]);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-                for (int f = 0; f < 4; ++f) {
-                    const int key = k0 + ty * 4 + e, row = q0 + tx * 4 + f;
-                    if (row < p.Nq && (!p.causal || key <= row + p.off))
-                        w[e] += exp2f(fmaf(s[e][f], p.scale_log2, -slse[tx * 4 + f]));
+                for (int kk = 0; kk < D / 16; ++kk) {
+                    const uint32_t o = (kk >> 2) * Cfg::kBox + (kk & 3) * 32;
+                    umma_f16_ss(tmem + bf * 128, smem_desc_sw128(sK + o, 16, 1024), smem_desc_sw128(sQ(st) + o, 16, 1024),
+                                id, kk > 0);
                 }
+                umma_commit(bar_q_empty(st));
+                umma_commit(bar_s_full(bf));
+            }
+            umma_commit(bar_done);
+            mbar_wait(bar_done, 0, kSiteKwDone, &no_abort);
+        }
+    } else if (warp == Cfg::kLseWarp) {
+        // -lse of the tile's queries in log2; -inf where the row saw no key.  Four buffers: the epilogue has let go of S tile it - 2
+        // only after it was done with tile it - 3.
+        auto fetch = [&](int it, float (&v)[4]) {
+            int h, q0;
+            tile_of(it, h, q0);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const int r = q0 + e * 32 + lane;
+                const float l = r < p.Nq ? __ldg(p.lse + b * p.l_sb + h * p.l_sh + r) : -INFINITY;
+                v[e] = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
+            }
+        };
+        float v[4];
+        if (n_it > 0) fetch(0, v);
+        for (int it = 0; it < n_it; ++it) {
+            if (it >= 2 && !mbar_wait(bar_s_empty(it & 1), ((it >> 1) - 1) & 1, kSiteKwSEmpty, abort_flag)) break;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s_lse[(it & 3) * 128 + e * 32 + lane] = v[e];
+            if (it + 1 < n_it) fetch(it + 1, v);
+            mbar_arrive(bar_s_full(it & 1));
+        }
+    } else {
+        // --------------------------------- epilogue: thread = key, half the columns
+        const int half = warp >> 2, key = (warp & 3) * 32 + lane;
+        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
+        for (int it = 0; it < n_it; ++it) {
+            const int bf = it & 1;
+            if (!mbar_wait(bar_s_full(bf), (it >> 1) & 1, kSiteKwS, abort_flag)) break;
+            tc_fence_after();
+            uint32_t r0[32], r1[32];
+            tmem_ld32(tmem + lane_off + bf * 128 + half * 64, r0);
+            tmem_ld32(tmem + lane_off + bf * 128 + half * 64 + 32, r1);
+            tmem_wait_ld();
+            tc_fence_before();
+            mbar_arrive(bar_s_empty(bf));
+            int h, q0;
+            tile_of(it, h, q0);
+            const uint32_t sl = base + Cfg::kOffLse + ((it & 3) * 128 + half * 64) * 4;
+            // columns [0, lo) are queries before this key
+            const int64_t before = p.causal ? (int64_t)j * 128 + key - p.off - q0 : 0;
+            const int lo = (int)max64(-1, min64(128, before)) - half * 64;
+            // columns [hi, 64) are no queries (their rows are zeros: a NaN key would reach the sum)
+            const int hi = min(128, p.Nq - q0) - half * 64;
+            uint64_t acc[4] = {};
+            // a warp whose every key is seen by every query of its columns needs no mask
+            if (__all_sync(0xffffffffu, lo <= 0 && hi >= 64)) {
+#pragma unroll
+                for (int e = 0; e < 32; e += 2) {
+                    uint64_t n0, n1;
+                    asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(n0), "=l"(n1) : "r"(sl + e * 8));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        const uint32_t *r = e < 16 ? r0 : r1;
+                        const int c = (2 * (e + u)) & 31;
+                        const uint64_t x =
+                            f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, u ? n1 : n0);
+                        uint64_t w;
+                        if ((e + u) % kKwPolyPeriod == kKwPolyPeriod - 1) {
+                            w = exp2_poly5_x2(x);
+                        } else {
+                            float x0, x1;
+                            f2_unpack(x, x0, x1);
+                            w = f2_pack(ex2_approx(x0), ex2_approx(x1));
+                        }
+                        acc[(e + u) & 3] = f2_add(acc[(e + u) & 3], w);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int e = 0; e < 32; ++e) {
+                    uint64_t n0;
+                    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(n0) : "r"(sl + e * 8));
+                    const uint32_t *r = e < 16 ? r0 : r1;
+                    const int c = (2 * e) & 31;
+                    float x0, x1;
+                    f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, n0), x0, x1);
+                    const float w0 = 2 * e >= lo && 2 * e < hi ? ex2_approx(x0) : 0.f;
+                    const float w1 = 2 * e + 1 >= lo && 2 * e + 1 < hi ? ex2_approx(x1) : 0.f;
+                    acc[e & 3] = f2_add(acc[e & 3], f2_pack(w0, w1));
+                }
+            }
+            // a tile's sum first, then the total: the longest chains stay short
+            float a, c;
+            f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a, c);
+            total += a + c;
+        }
+        if (half == 1) s_red[key] = total;
+    }
+    __syncthreads();
+    if (warp < 4) {
+        const int key = warp * 32 + lane;
+        const int64_t c = (int64_t)j * 128 + key;
+        if (c < p.Nkv) {
+            const float w = total + s_red[key];
+            if (p.part) {
+                p.out[split * p.part + ((int64_t)b * p.Hkv + hk) * p.Nkv + c] = w;
+            } else {
+                float *o = p.out + b * p.o_sb + hk * p.o_sh + c;
+                *o = p.accumulate ? *o + w : w;
+            }
         }
     }
-#pragma unroll
-    for (int e = 0; e < 4; ++e) red[ty * 4 + e][tx] = w[e];
-    __syncthreads();
-    if (threadIdx.x < 64 && k0 + threadIdx.x < p.Nkv) {
-        float t = 0.f;
-        for (int x = 0; x < 16; ++x) t += red[threadIdx.x][x];
-        float *o = p.out + b * p.o_sb + hk * p.o_sh + k0 + threadIdx.x;
-        *o = p.accumulate ? *o + t : t;
+    if (warp == Cfg::kMmaWarp) {
+        tc_fence_after();
+        tmem_dealloc(tmem, Cfg::kTmemCols);
     }
+}
+
+// Adds the splits' parts in their order.
+__global__ void key_weights_sum_kernel(const float *parts, float *out, int64_t o_sb, int64_t o_sh, int Hkv, int Nkv,
+                                       int64_t part, int splits, int accumulate) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i >= part) return;
+    float w = 0.f;
+    for (int s = 0; s < splits; ++s) w += parts[s * part + i];
+    const int64_t row = i / Nkv;
+    float *o = out + row / Hkv * o_sb + row % Hkv * o_sh + i % Nkv;
+    *o = accumulate ? *o + w : w;
+}
+
+// A block without queries: nothing to add, or zeros.
+__global__ void key_weights_zero_kernel(float *out, int64_t o_sb, int64_t o_sh, int Hkv, int Nkv, int64_t n) {
+    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    if (i < n) out[i / Nkv / Hkv * o_sb + i / Nkv % Hkv * o_sh + i % Nkv] = 0.f;
 }
 
 }  // namespace gae

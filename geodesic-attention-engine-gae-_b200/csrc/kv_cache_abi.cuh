@@ -74,6 +74,25 @@ PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool
     return w;
 }
 
+// How many CTAs share a key tile's queries.  One where the key tiles fill the
+// GPU (two CTAs to an SM); else enough to fill it, as long as each is left with
+// 4 query tiles.
+int key_weights_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nkv) {
+    const int64_t units = B * Hkv * ((Nkv + 127) / 128), tiles = H / Hkv * ((Nq + 127) / 128);
+    const int64_t want = (2 * num_sms() + units - 1) / units;
+    return (int)gae::max64(1, gae::min64(want, tiles / 4));
+}
+
+template <int D, bool kBF16>
+gae_status launch_key_weights(const gae::KeyWeightsParams &p, dim3 grid, cudaStream_t st) {
+    using Cfg = gae::KeyWeightsCfg<D>;
+    gae_status s = set_smem(gae::key_weights_kernel<D, kBF16>, Cfg::kSmem);
+    if (s != GAE_OK) return s;
+    gae::key_weights_kernel<D, kBF16><<<grid, Cfg::kThreads, Cfg::kSmem, st>>>(p);
+    GAE_CUDA_TRY(cudaGetLastError());
+    return GAE_OK;
+}
+
 // A launch that may begin while the one before it ends (it waits for it by griddepcontrol.wait).
 template <typename... Params, typename... Args>
 gae_status launch_after(void (*kern)(Params...), dim3 grid, int threads, cudaStream_t st, Args... args) {
@@ -227,8 +246,11 @@ gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args
 }
 
 size_t gae_key_weights_workspace_bytes(int64_t batch, int64_t heads, int64_t kv_heads, int64_t seq_q, int64_t seq_kv) {
-    (void)batch; (void)heads; (void)kv_heads; (void)seq_q; (void)seq_kv;
-    return 0;
+    if (batch < 1 || heads < 1 || kv_heads < 1 || seq_q < 1 || seq_kv < 1 || heads % kv_heads ||
+        batch * heads > 65535 || seq_q > kMaxPositions || seq_kv > kMaxPositions)
+        return 0;
+    const int splits = key_weights_splits(batch, heads, kv_heads, seq_q, seq_kv);
+    return splits == 1 ? 0 : (size_t)splits * batch * kv_heads * seq_kv * 4;
 }
 
 gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
@@ -252,30 +274,53 @@ gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
     for (int i = 0; i < 2; ++i)
         if (a->lse_stride[i] < 0 || a->out_stride[i] < 0)
             return fail(GAE_ERR_INVALID_ARG, "negative lse or out stride");
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (a->seq_q == 0) {
+        const int64_t n = a->batch * a->kv_heads * a->seq_kv, blocks = (n + 255) / 256;
+        if (a->accumulate) return GAE_OK;
+        if (blocks > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many keys");
+        gae::key_weights_zero_kernel<<<(unsigned)blocks, 256, 0, st>>>(a->out, a->out_stride[0], a->out_stride[1],
+                                                                       (int)a->kv_heads, (int)a->seq_kv, n);
+        GAE_CUDA_TRY(cudaGetLastError());
+        return GAE_OK;
+    }
+    const size_t need = gae_key_weights_workspace_bytes(a->batch, a->heads, a->kv_heads, a->seq_q, a->seq_kv);
+    if (a->workspace_bytes < need || (need && (!a->workspace || !aligned16(a->workspace))))
+        return fail(GAE_ERR_INVALID_ARG, "workspace too small or not 16-byte aligned: %zu < %zu", a->workspace_bytes, need);
     gae::KeyWeightsParams p;
     memset(&p, 0, sizeof(p));
-    p.q = a->q; p.k = a->k; p.lse = a->lse; p.out = a->out;
-    p.q_sb = a->q_stride[0]; p.q_sh = a->q_stride[1]; p.q_ss = a->q_stride[2];
-    p.k_sb = a->k_stride[0]; p.k_sh = a->k_stride[1]; p.k_ss = a->k_stride[2];
+    gae_status s;
+    const bool bf16 = a->dtype == GAE_DTYPE_BF16;
+    const int64_t D = a->head_dim;
+    const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if ((s = make_map_4d(&p.tm_q, a->q, dt, 2, a->batch, a->heads, a->seq_q, D, a->q_stride[0], a->q_stride[1],
+                         a->q_stride[2], 128)) != GAE_OK ||
+        (s = make_map_4d(&p.tm_k, a->k, dt, 2, a->batch, a->kv_heads, a->seq_kv, D, a->k_stride[0], a->k_stride[1],
+                         a->k_stride[2], 128)) != GAE_OK)
+        return s;
+    p.lse = a->lse;
     p.l_sb = a->lse_stride[0]; p.l_sh = a->lse_stride[1];
     p.o_sb = a->out_stride[0]; p.o_sh = a->out_stride[1];
     p.B = (int)a->batch; p.H = (int)a->heads; p.Hkv = (int)a->kv_heads;
-    p.Nq = (int)a->seq_q; p.Nkv = (int)a->seq_kv; p.D = (int)a->head_dim;
+    p.Nq = (int)a->seq_q; p.Nkv = (int)a->seq_kv;
     p.causal = a->causal ? 1 : 0;
     p.accumulate = a->accumulate ? 1 : 0;
-    p.off = a->q_offset - a->kv_offset;
+    // Beyond the longest sequence all offsets mean the same.
+    const __int128 off = (__int128)a->q_offset - a->kv_offset, most = 2 * (__int128)kMaxPositions;
+    p.off = (int64_t)(off > most ? most : off < -most ? -most : off);
     p.scale_log2 = a->scale * 1.4426950408889634f;
-    const dim3 grid((unsigned)((a->seq_kv + 63) / 64), (unsigned)a->kv_heads, (unsigned)a->batch);
-    const int smem = 2 * 64 * (p.D + 1) * 4;
-    cudaStream_t st = static_cast<cudaStream_t>(stream);
-    gae_status s;
-    if (a->dtype == GAE_DTYPE_BF16) {
-        if ((s = set_smem(gae::key_weights_kernel<__nv_bfloat16>, smem)) != GAE_OK) return s;
-        gae::key_weights_kernel<__nv_bfloat16><<<grid, 256, smem, st>>>(p);
-    } else {
-        if ((s = set_smem(gae::key_weights_kernel<__half>, smem)) != GAE_OK) return s;
-        gae::key_weights_kernel<__half><<<grid, 256, smem, st>>>(p);
-    }
+    p.splits = key_weights_splits(a->batch, a->heads, a->kv_heads, a->seq_q, a->seq_kv);
+    p.part = p.splits > 1 ? a->batch * a->kv_heads * a->seq_kv : 0;
+    p.out = p.splits > 1 ? static_cast<float *>(a->workspace) : a->out;
+    const int64_t units = a->batch * a->kv_heads * ((a->seq_kv + 127) / 128);
+    if (units > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many key tiles");
+    const dim3 grid((unsigned)units, (unsigned)p.splits);
+    if (D == 128) s = bf16 ? launch_key_weights<128, true>(p, grid, st) : launch_key_weights<128, false>(p, grid, st);
+    else s = bf16 ? launch_key_weights<64, true>(p, grid, st) : launch_key_weights<64, false>(p, grid, st);
+    if (s != GAE_OK || p.splits == 1) return s;
+    const int64_t blocks = (p.part + 255) / 256;
+    gae::key_weights_sum_kernel<<<(unsigned)blocks, 256, 0, st>>>(p.out, a->out, p.o_sb, p.o_sh, p.Hkv, p.Nkv, p.part,
+                                                                  p.splits, p.accumulate);
     GAE_CUDA_TRY(cudaGetLastError());
     return GAE_OK;
 }
