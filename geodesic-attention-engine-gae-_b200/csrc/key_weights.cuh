@@ -11,8 +11,8 @@
 // its key's weights in registers and no two threads ever share a sum (no
 // atomics, the same bits every time).  One CTA per (128-key tile, key head,
 // batch): K stays in shared memory, the tiles of 128 queries of all the head's
-// query heads stream through a TMA ring, two S tiles alternate in TMEM so that
-// the next product runs while eight warps exponentiate the last.  Two CTAs to
+// query heads stream through a TMA ring, two S tiles alternate in TMEM, each
+// with a warpgroup of its own that exponentiates it while the other's product runs.  Two CTAs to
 // an SM.
 //
 // What bounds it: one exponential per score.  The MUFU gives 16 a cycle and
@@ -42,7 +42,7 @@ enum KeyWeightsWaitSite : unsigned {
 };
 
 #ifndef GAE_KW_POLY_PERIOD
-#define GAE_KW_POLY_PERIOD 2
+#define GAE_KW_POLY_PERIOD 4
 #endif
 constexpr int kKwPolyPeriod = GAE_KW_POLY_PERIOD;
 
@@ -79,12 +79,12 @@ struct KeyWeightsCfg {
     static constexpr int kBox = 128 * 128, kPanels = D * 2 / 128, kTile = kPanels * kBox;
     static constexpr int kStages = D == 128 ? 2 : 4;
     static constexpr int kOffK = 0, kOffQ = kTile, kOffLse = kOffQ + kStages * kTile;  // lse: 4 tiles of 128
-    static constexpr int kOffRed = kOffLse + 4 * 128 * 4;                               // 128 sums of the upper columns
+    static constexpr int kOffRed = kOffLse + 4 * 128 * 4;                               // 128 sums of the second warpgroup
     static constexpr int kOffBar = kOffRed + 128 * 4;
     static constexpr int kNumBars = 2 + 2 * kStages + 4;  // k, done, q_full/q_empty, s_full/s_empty [2]
     static constexpr int kPayload = kOffBar + kNumBars * 8 + 16;
     static constexpr int kSmem = kPayload + 1024;  // slack for the 1024-byte alignment of the swizzle atoms
-    static constexpr int kEpiWarps = 8, kTmaWarp = 8, kMmaWarp = 9, kLseWarp = 10, kThreads = 11 * 32;
+    static constexpr int kTmaWarp = 8, kMmaWarp = 9, kLseWarp = 10, kThreads = 11 * 32;
     static constexpr uint32_t kTmemCols = 256;
     static_assert(2 * (kSmem + 1024) <= 228 * 1024, "two CTAs to an SM");
 };
@@ -122,10 +122,11 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
     const int per_head = nq - i0, all = per_head * G;
     const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
     const int n_it = t1 - t0;
-    auto tile_of = [&](int it, int &h, int &q0) {  // query tile it of this CTA
-        const int t = t0 + it;
-        h = hk * G + t / per_head;
-        q0 = (i0 + t % per_head) * 128;
+    // The query tile at hand: head h, tile i of those that see this key tile.
+    int h = hk * G, i = 0;
+    if (n_it > 0) h += t0 / per_head, i = t0 % per_head;
+    auto next_tile = [&] {
+        if (++i == per_head) i = 0, ++h;
     };
 
     if (threadIdx.x == 0) {
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
         }
         for (int bf = 0; bf < 2; ++bf) {
             mbar_init(bar_s_full(bf), 1 + 32);  // the products, and the lanes of the lse warp
-            mbar_init(bar_s_empty(bf), Cfg::kEpiWarps * 32);
+            mbar_init(bar_s_empty(bf), 128);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -162,11 +163,10 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             for (; it < n_it; ++it) {
                 const int st = it % Cfg::kStages, use = it / Cfg::kStages;
                 if (use > 0 && !mbar_wait(bar_q_empty(st), (use - 1) & 1, kSiteKwQEmpty, abort_flag)) break;
-                int h, q0;
-                tile_of(it, h, q0);
                 mbar_expect_tx(bar_q_full(st), Cfg::kTile);
                 for (int hf = 0; hf < Cfg::kPanels; ++hf)
-                    tma_load_4d(sQ(st) + hf * Cfg::kBox, &p.tm_q, bar_q_full(st), hf * 64, q0, h, b);
+                    tma_load_4d(sQ(st) + hf * Cfg::kBox, &p.tm_q, bar_q_full(st), hf * 64, (i0 + i) * 128, h, b);
+                next_tile();
             }
             // the copies issued have landed before the CTA exits
             mbar_wait(bar_k, 0, kSiteKwK, &no_abort);
@@ -195,86 +195,92 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             mbar_wait(bar_done, 0, kSiteKwDone, &no_abort);
         }
     } else if (warp == Cfg::kLseWarp) {
-        // -lse of the tile's queries in log2; -inf where the row saw no key.  Four buffers: the epilogue has let go of S tile it - 2
-        // only after it was done with tile it - 3.
-        auto fetch = [&](int it, float (&v)[4]) {
-            int h, q0;
-            tile_of(it, h, q0);
+        // -lse of the tile's queries in log2; -inf where the row saw no key.  Four
+        // buffers: the warpgroup that has let go of S tile it - 2 is done with
+        // tile it - 4.
+        auto fetch = [&](float (&v)[4]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int r = q0 + e * 32 + lane;
+                const int r = (i0 + i) * 128 + e * 32 + lane;
                 const float l = r < p.Nq ? __ldg(p.lse + b * p.l_sb + h * p.l_sh + r) : -INFINITY;
                 v[e] = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
             }
+            next_tile();
         };
         float v[4];
-        if (n_it > 0) fetch(0, v);
+        if (n_it > 0) fetch(v);
         for (int it = 0; it < n_it; ++it) {
             if (it >= 2 && !mbar_wait(bar_s_empty(it & 1), ((it >> 1) - 1) & 1, kSiteKwSEmpty, abort_flag)) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) s_lse[(it & 3) * 128 + e * 32 + lane] = v[e];
-            if (it + 1 < n_it) fetch(it + 1, v);
+            if (it + 1 < n_it) fetch(v);
             mbar_arrive(bar_s_full(it & 1));
         }
     } else {
-        // --------------------------------- epilogue: thread = key, half the columns
-        const int half = warp >> 2, key = (warp & 3) * 32 + lane;
-        const uint32_t lane_off = (uint32_t)((warp & 3) * 32) << 16;
+        // -------------- epilogue: warpgroup g takes every second S tile, thread = key
+        const int g = warp >> 2, key = (warp & 3) * 32 + lane;
+        const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 128;
         const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
-        for (int it = 0; it < n_it; ++it) {
-            const int bf = it & 1;
-            if (!mbar_wait(bar_s_full(bf), (it >> 1) & 1, kSiteKwS, abort_flag)) break;
+        // Columns before this are queries before this thread's (this warp's last)
+        // key, for the first query tile; beyond it every tile moves it by 128.
+        const int64_t first = p.causal ? (int64_t)j * 128 + key - p.off : INT64_MIN / 2;
+        const int64_t first_warp = first + 31 - lane;
+        if (g == 1) next_tile();
+        for (int it = g; it < n_it; it += 2) {
+            const int q0 = (i0 + i) * 128;
+            next_tile();
+            next_tile();
+            if (!mbar_wait(bar_s_full(g), (it >> 1) & 1, kSiteKwS, abort_flag)) break;
             tc_fence_after();
-            uint32_t r0[32], r1[32];
-            tmem_ld32(tmem + lane_off + bf * 128 + half * 64, r0);
-            tmem_ld32(tmem + lane_off + bf * 128 + half * 64 + 32, r1);
-            tmem_wait_ld();
-            tc_fence_before();
-            mbar_arrive(bar_s_empty(bf));
-            int h, q0;
-            tile_of(it, h, q0);
-            const uint32_t sl = base + Cfg::kOffLse + ((it & 3) * 128 + half * 64) * 4;
-            // columns [0, lo) are queries before this key
-            const int64_t before = p.causal ? (int64_t)j * 128 + key - p.off - q0 : 0;
-            const int lo = (int)max64(-1, min64(128, before)) - half * 64;
-            // columns [hi, 64) are no queries (their rows are zeros: a NaN key would reach the sum)
-            const int hi = min(128, p.Nq - q0) - half * 64;
+            const uint32_t sl = base + Cfg::kOffLse + (it & 3) * 512;
             uint64_t acc[4] = {};
-            // a warp whose every key is seen by every query of its columns needs no mask
-            if (__all_sync(0xffffffffu, lo <= 0 && hi >= 64)) {
+            // a warp whose every key is seen by all 128 queries needs no mask
+            const bool full = first_warp <= q0 && q0 + 128 <= p.Nq;
+            // columns [lo, hi) count; those from hi on are no queries (their rows
+            // are zeros: a NaN key would reach the sum)
+            const int lo = (int)max64(0, min64(128, first - q0)), hi = min(128, p.Nq - q0);
 #pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    uint64_t n0, n1;
-                    asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(n0), "=l"(n1) : "r"(sl + e * 8));
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        const uint32_t *r = e < 16 ? r0 : r1;
-                        const int c = (2 * (e + u)) & 31;
-                        const uint64_t x =
-                            f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, u ? n1 : n0);
-                        uint64_t w;
-                        if ((e + u) % kKwPolyPeriod == kKwPolyPeriod - 1) {
-                            w = exp2_poly5_x2(x);
-                        } else {
-                            float x0, x1;
-                            f2_unpack(x, x0, x1);
-                            w = f2_pack(ex2_approx(x0), ex2_approx(x1));
-                        }
-                        acc[(e + u) & 3] = f2_add(acc[(e + u) & 3], w);
-                    }
+            for (int c0 = 0; c0 < 128; c0 += 32) {
+                uint32_t r[32];
+                tmem_ld32(tS + c0, r);
+                tmem_wait_ld();
+                if (c0 == 96) {
+                    tc_fence_before();
+                    mbar_arrive(bar_s_empty(g));
                 }
-            } else {
+                if (full) {
 #pragma unroll
-                for (int e = 0; e < 32; ++e) {
-                    uint64_t n0;
-                    asm volatile("ld.shared.b64 %0, [%1];" : "=l"(n0) : "r"(sl + e * 8));
-                    const uint32_t *r = e < 16 ? r0 : r1;
-                    const int c = (2 * e) & 31;
-                    float x0, x1;
-                    f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, n0), x0, x1);
-                    const float w0 = 2 * e >= lo && 2 * e < hi ? ex2_approx(x0) : 0.f;
-                    const float w1 = 2 * e + 1 >= lo && 2 * e + 1 < hi ? ex2_approx(x1) : 0.f;
-                    acc[e & 3] = f2_add(acc[e & 3], f2_pack(w0, w1));
+                    for (int e = 0; e < 16; e += 2) {
+                        uint64_t n[2];
+                        asm volatile("ld.shared.v2.b64 {%0,%1}, [%2];" : "=l"(n[0]), "=l"(n[1]) : "r"(sl + c0 * 4 + e * 8));
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            const int c = 2 * (e + u);
+                            const uint64_t x =
+                                f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, n[u]);
+                            uint64_t w;
+                            if ((e + u) % kKwPolyPeriod == kKwPolyPeriod - 1) {
+                                w = exp2_poly5_x2(x);
+                            } else {
+                                float x0, x1;
+                                f2_unpack(x, x0, x1);
+                                w = f2_pack(ex2_approx(x0), ex2_approx(x1));
+                            }
+                            acc[(e + u) & 3] = f2_add(acc[(e + u) & 3], w);
+                        }
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) {
+                        uint64_t n0;
+                        asm volatile("ld.shared.b64 %0, [%1];" : "=l"(n0) : "r"(sl + c0 * 4 + e * 8));
+                        const int c = c0 + 2 * e;
+                        float x0, x1;
+                        f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), sl2, n0), x0, x1);
+                        const float w0 = c >= lo && c < hi ? ex2_approx(x0) : 0.f;
+                        const float w1 = c + 1 >= lo && c + 1 < hi ? ex2_approx(x1) : 0.f;
+                        acc[e & 3] = f2_add(acc[e & 3], f2_pack(w0, w1));
+                    }
                 }
             }
             // a tile's sum first, then the total: the longest chains stay short
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a, c);
             total += a + c;
         }
-        if (half == 1) s_red[key] = total;
+        if (g == 1) s_red[key] = total;
     }
     __syncthreads();
     if (warp < 4) {
