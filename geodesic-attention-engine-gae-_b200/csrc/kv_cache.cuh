@@ -66,33 +66,50 @@ struct AppendParams {
     int64_t kn_sb, kn_sh, kn_st, vn_sb, vn_sh, vn_st;  // element strides: batch, head, token
     const int *start, *counts;                         // counts may be NULL: all tokens
     int tokens, chunks;                                // chunks: 16-byte pieces of a row
+    FastDiv by_chunks, by_heads;
 };
 
-// One thread per 16-byte piece of a new row, K and V both.
+// A thread copies 16 bytes of kAppendRows new rows, K and V both; all of its
+// reads are on their way before it writes (one row to a thread keeps a 335 MB
+// prompt at 66 us, four bring it to the copy rate).
+constexpr int kAppendRows = 4;
+
 template <int ESIZE>
-__global__ void paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
     const int b = blockIdx.y;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int c = (int)(i % p.chunks);
-    const int h = (int)(i / p.chunks % p.pool.Hkv);
-    const int64_t t = i / p.chunks / p.pool.Hkv;
-    const int n = p.counts ? min(p.counts[b], p.tokens) : p.tokens;
-    if (t >= n) return;
-    const int64_t pos = (int64_t)p.start[b] + t;
-    if (pos < 0 || pos >= (int64_t)p.table.max_pages * p.pool.page) return;
-    const int pg = page_of(p.table, p.pool.num_pages, b, (int)(pos / p.pool.page));
-    if (pg < 0) return;
-    const int64_t slot = pos % p.pool.page;
-    const int4 *ks = reinterpret_cast<const int4 *>(static_cast<const char *>(p.k_new) +
-                                                    (b * p.kn_sb + h * p.kn_sh + t * p.kn_st) * ESIZE);
-    const int4 *vs = reinterpret_cast<const int4 *>(static_cast<const char *>(p.v_new) +
-                                                    (b * p.vn_sb + h * p.vn_sh + t * p.vn_st) * ESIZE);
-    int4 *kd = reinterpret_cast<int4 *>(static_cast<char *>(p.pool.k) +
-                                        (pg * p.pool.k_sp + h * p.pool.k_sh + slot * p.pool.k_ss) * ESIZE);
-    int4 *vd = reinterpret_cast<int4 *>(static_cast<char *>(p.pool.v) +
-                                        (pg * p.pool.v_sp + h * p.pool.v_sh + slot * p.pool.v_ss) * ESIZE);
-    kd[c] = __ldg(ks + c);
-    vd[c] = __ldg(vs + c);
+    const int n = p.counts ? min(p.counts[b], p.tokens) : p.tokens, start = p.start[b];
+    const int64_t cap = (int64_t)p.table.max_pages * p.pool.page;
+    int64_t k_to[kAppendRows], v_to[kAppendRows];
+    int4 x[kAppendRows], y[kAppendRows];
+    bool live[kAppendRows];
+#pragma unroll
+    for (int e = 0; e < kAppendRows; ++e) {
+        const uint32_t i = ((uint32_t)blockIdx.x * kAppendRows + e) * 256u + threadIdx.x;
+        const uint32_t row = p.by_chunks.div(i), t = p.by_heads.div(row);
+        const int c = (int)(i - row * p.chunks), h = (int)(row - t * p.pool.Hkv);
+        const int64_t pos = (int64_t)start + t;
+        live[e] = (int64_t)t < n && pos >= 0 && pos < cap;
+        int pg = -1;
+        int64_t slot = 0;
+        if (live[e]) {
+            const uint32_t idx = p.pool.by_page.div((uint32_t)pos);
+            pg = page_of(p.table, p.pool.num_pages, b, (int)idx);
+            slot = pos - (int64_t)idx * p.pool.page;
+            x[e] = __ldg(reinterpret_cast<const int4 *>(static_cast<const char *>(p.k_new) +
+                                                       (b * p.kn_sb + h * p.kn_sh + t * p.kn_st) * ESIZE) + c);
+            y[e] = __ldg(reinterpret_cast<const int4 *>(static_cast<const char *>(p.v_new) +
+                                                       (b * p.vn_sb + h * p.vn_sh + t * p.vn_st) * ESIZE) + c);
+        }
+        live[e] = pg >= 0;
+        k_to[e] = (pg * p.pool.k_sp + h * p.pool.k_sh + slot * p.pool.k_ss) * ESIZE + c * 16;
+        v_to[e] = (pg * p.pool.v_sp + h * p.pool.v_sh + slot * p.pool.v_ss) * ESIZE + c * 16;
+    }
+#pragma unroll
+    for (int e = 0; e < kAppendRows; ++e)
+        if (live[e]) {
+            *reinterpret_cast<int4 *>(static_cast<char *>(p.pool.k) + k_to[e]) = x[e];
+            *reinterpret_cast<int4 *>(static_cast<char *>(p.pool.v) + v_to[e]) = y[e];
+        }
 }
 
 // ---------------------------------------------------------------- eviction
@@ -118,100 +135,271 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
-__device__ __forceinline__ uint32_t evict_key(const EvictParams &p, int b, int hk, int pos, int len) {
-    if (page_of(p.src, p.pool.num_pages, b, pos / p.pool.page) < 0) return 0u;
-    if (pos >= len - p.recent) return 0xffffffffu;
-    return weight_key(__ldg(p.w + b * p.w_sb + hk * p.w_sh + pos));
+// The keep-th largest key of a (key head, sequence) row is found by a radix
+// search over its 11, 11 and 10 highest bits; positions above it, and the first
+// of those equal to it, are then listed in ascending order.  A cluster of up to
+// 8 CTAs shares a row where there are few rows, each with its run of positions: the keys are formed once
+// and stay in shared memory (positions beyond kMaxKeys are formed again), only
+// histograms and counts cross the cluster.  What bounds it is latency: one
+// barrier of the cluster to a digit.
+#ifndef GAE_EV_THREADS
+#define GAE_EV_THREADS 1024
+#endif
+constexpr int kEvictThreads = GAE_EV_THREADS, kEvictWarps = kEvictThreads / 32, kEvictBins = 2048;
+constexpr int kEvictMaxCluster = 8, kEvictMaxKeys = 40960;
+
+// A cluster barrier after which the CTAs see what the others wrote before it:
+// one thread's fence stands for the CTA (its threads have met before), where a
+// releasing arrival would be a fence of every thread.
+__device__ __forceinline__ void cluster_publish() {
+    __syncthreads();
+    if (threadIdx.x == 0) asm volatile("fence.acq_rel.cluster;" ::: "memory");
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+__device__ __forceinline__ uint2 ld_cluster_u2(uint32_t addr, uint32_t rank) {
+    uint2 v;
+    asm volatile("ld.shared::cluster.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(mapa_shared(addr, rank)) : "memory");
+    return v;
 }
 
-// One CTA per (kv head, sequence).  The keep-th largest key is found by four
-// passes over its 8-bit digits; positions above it, and the first of those
-// equal to it, are listed in ascending order.
-__global__ void __launch_bounds__(1024) evict_select_kernel(const EvictParams p) {
-    const int hk = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictParams p, int cluster, int max_keys) {
+    extern __shared__ __align__(16) uint32_t smem_ev[];
+    uint32_t *hist = smem_ev;                    // [2][bins], one digit's after the other's
+    uint32_t *keys = smem_ev + 2 * kEvictBins;  // [max_keys], a multiple of 4
+    __shared__ uint32_t s_warp[kEvictWarps], s_digit, s_left;
+    __shared__ __align__(8) uint32_t s_counts[2];
+    const int rank = (int)cluster_ctarank(), row = blockIdx.x / cluster, hk = row % p.pool.Hkv, b = row / p.pool.Hkv;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int len = clamp_len(p.lens[b], p.cap);
-    __shared__ int hist[256];
-    __shared__ uint32_t s_prefix;
-    __shared__ int s_left, s_total, s_gt[32], s_eq[32];
-    // Keys that may be kept.
-    int mine = 0;
-    for (int i = tid; i < len; i += 1024) mine += evict_key(p, b, hk, i, len) != 0u;
-    if (tid == 0) s_total = 0;
-    __syncthreads();
-    atomicAdd(&s_total, mine);
-    __syncthreads();
-    const int n_keep = min(p.keep, s_total);
-    uint32_t prefix = 0;
-    int left = n_keep;  // how many of the keys that share the prefix are kept
-    for (int shift = 24; shift >= 0 && n_keep > 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < len; i += 1024) {
-            const uint32_t k = evict_key(p, b, hk, i, len);
-            if (k != 0u && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))))
-                atomicAdd(&hist[(k >> shift) & 255], 1);
+    const int per = (len + cluster - 1) / cluster, lo = min(len, rank * per), n = min(len, lo + per) - lo;
+    const float *w = p.w + b * p.w_sb + hk * p.w_sh + lo;
+    const int *table = p.src.entry + b * p.src.stride;
+    const int pages = (int)p.pool.num_pages, forced = len - p.recent - lo;
+    auto key_of = [&](int i, int pg, float x) -> uint32_t {
+        return (uint32_t)pg >= (uint32_t)pages ? 0u : i >= forced ? 0xffffffffu : weight_key(x);
+    };
+    auto form = [&](int i) -> uint32_t {  // the key of this CTA's position i
+        return key_of(i, __ldg(table + p.pool.by_page.div(lo + i)), __ldg(w + i));
+    };
+    const bool all_held = n <= max_keys;
+    auto get4 = [&](int i, uint32_t (&k)[4]) {  // keys i .. i + 3, 0 beyond the end; i a multiple of 4
+        if (all_held) {
+            const uint4 v = *reinterpret_cast<const uint4 *>(keys + i);
+            k[0] = v.x, k[1] = v.y, k[2] = v.z, k[3] = v.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k[e] = i + e >= n ? 0u : i + e < max_keys ? keys[i + e] : form(i + e);
         }
-        __syncthreads();
-        if (tid == 0) {
-            int d = 255, n = left;
-            while (d > 0 && hist[d] < n) n -= hist[d--];
-            s_prefix = prefix | ((uint32_t)d << shift);
-            s_left = n;
+    };
+    for (int i = tid; i < 2 * kEvictBins; i += kEvictThreads) hist[i] = 0;
+    const int held = min(n, max_keys);
+    for (int i0 = tid; i0 < held; i0 += 8 * kEvictThreads) {  // eight pages and weights on their way at once
+        int pg[8];
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = min(i0 + e * kEvictThreads, held - 1);
+            pg[e] = __ldg(table + p.pool.by_page.div(lo + i));
+            x[e] = __ldg(w + i);
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int i = i0 + e * kEvictThreads;
+            if (i < held) keys[i] = key_of(i, pg[e], x[e]);
+        }
+    }
+    if (tid < (-held & 3)) keys[held + tid] = 0;
+    uint32_t prefix = 0, left = 0;
+    int n_keep = 0;
+#pragma unroll 1
+    for (int digit = 0; digit < 3; ++digit) {
+        const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0;
+        const uint32_t mask = digit == 2 ? 1023u : 2047u;
+        // the bits above this digit have to be the prefix's
+        const uint32_t above = digit == 0 ? 0u : digit == 1 ? 0xffe00000u : 0xfffffc00u;
+        uint32_t *h = hist + (digit & 1) * kEvictBins;
         __syncthreads();
-        prefix = s_prefix;
+        for (int i = tid * 4; i < n; i += kEvictThreads * 4) {
+            uint32_t k[4];
+            get4(i, k);
+            // few keys share the upper digits: mostly none of four
+            uint32_t off = 0xffffffffu;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) off = min(off, (k[e] ^ prefix) & above);
+            if (off == 0u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (k[e] != 0u && ((k[e] ^ prefix) & above) == 0u) atomicAdd(h + ((k[e] >> shift) & mask), 1u);
+        }
+        cluster_publish();
+        // Every CTA adds up the whole cluster's bins, kBins to a thread from the top.
+        constexpr int kBins = kEvictBins / kEvictThreads;
+        const uint32_t ha = smem_u32(h) + (kEvictBins - (tid + 1) * kBins) * 4;
+        uint32_t c[kBins] = {}, mine = 0;
+#pragma unroll
+        for (int r = 0; r < kEvictMaxCluster; ++r)
+            if (r < cluster)
+#pragma unroll
+                for (int e = 0; e < kBins; e += 2) {
+                    const uint2 x = ld_cluster_u2(ha + (kBins - 2 - e) * 4, (uint32_t)r);
+                    c[e] += x.y, c[e + 1] += x.x;
+                }
+#pragma unroll
+        for (int e = 0; e < kBins; ++e) mine += c[e];
+        uint32_t incl = mine;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const uint32_t up = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += up;
+        }
+        if (lane == 31) s_warp[warp] = incl;
+        __syncthreads();
+        const uint32_t sums = lane < kEvictWarps ? s_warp[lane] : 0u;
+        uint32_t before = incl - mine + __reduce_add_sync(0xffffffffu, lane < warp ? sums : 0u);
+        if (digit == 0) {
+            n_keep = min(p.keep, (int)__reduce_add_sync(0xffffffffu, sums));
+            left = (uint32_t)n_keep;
+        }
+        // the thread in whose bins the running count reaches `left`
+        if (before < left && before + mine >= left)
+#pragma unroll
+            for (int e = 0; e < kBins; ++e) {
+                if (before < left && before + c[e] >= left) {
+                    s_digit = kEvictBins - 1 - tid * kBins - e;
+                    s_left = left - before;
+                }
+                before += c[e];
+            }
+        __syncthreads();
+        if (n_keep == 0) break;  // the same in every CTA of the cluster
+        prefix |= s_digit << shift;
         left = s_left;
+        // The third digit uses the first one's bins: every CTA has read them once
+        // all have passed the second's barrier.
+        if (digit == 1)
+            for (int i = tid; i < kEvictBins; i += kEvictThreads) hist[i] = 0;
     }
+    // Keys above the threshold and equal to it: every warp a run of positions,
+    // counted, then listed from where the runs before it end.
+    const int run = (((n + kEvictWarps - 1) / kEvictWarps) + 127) / 128 * 128, first = warp * run, last = min(n, first + run);
+    uint32_t gt = 0, eq = 0;
+    if (n_keep > 0)
+        for (int i = first + lane * 4; i < last; i += 128) {
+            uint32_t k[4];
+            get4(i, k);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) gt += k[e] > prefix, eq += k[e] == prefix && k[e] != 0u;
+        }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
+    __shared__ uint32_t s_gt[kEvictWarps], s_eq[kEvictWarps];
+    if (lane == 0) s_gt[warp] = gt, s_eq[warp] = eq;
+    __syncthreads();
+    const uint32_t gts = lane < kEvictWarps ? s_gt[lane] : 0u, eqs = lane < kEvictWarps ? s_eq[lane] : 0u;
+    if (warp == 0) {
+        const uint32_t g = __reduce_add_sync(0xffffffffu, gts), e = __reduce_add_sync(0xffffffffu, eqs);
+        if (lane == 0) s_counts[0] = g, s_counts[1] = e;
+    }
+    cluster_publish();
+    uint32_t g0 = __reduce_add_sync(0xffffffffu, lane < warp ? gts : 0u);
+    uint32_t e0 = __reduce_add_sync(0xffffffffu, lane < warp ? eqs : 0u);
+#pragma unroll
+    for (int r = 0; r < kEvictMaxCluster - 1; ++r)
+        if (r < rank) {
+            const uint2 x = ld_cluster_u2(smem_u32(s_counts), (uint32_t)r);
+            g0 += x.x, e0 += x.y;
+        }
     int *kept = p.kept + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
-    float *wo = p.w_out + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
-    int done = 0, eq_done = 0;
-    for (int i0 = 0; i0 < len && n_keep > 0; i0 += 1024) {
-        const int i = i0 + tid;
-        const uint32_t k = i < len ? evict_key(p, b, hk, i, len) : 0u;
-        const bool gt = k > prefix, eq = k == prefix && k != 0u;
-        const unsigned bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-        __syncthreads();
-        if (lane == 0) s_gt[warp] = __popc(bg), s_eq[warp] = __popc(be);
-        __syncthreads();
-        int g = 0, e = 0, gall = 0, eall = 0;
-        for (int w = 0; w < 32; ++w) {
-            if (w < warp) g += s_gt[w], e += s_eq[w];
-            gall += s_gt[w], eall += s_eq[w];
+    if (n_keep > 0)
+        for (int i0 = first; i0 < last; i0 += 128) {
+            const int i = i0 + lane * 4;
+            uint32_t k[4] = {};
+            if (i < last) get4(i, k);
+            uint32_t mine = 0;  // above in the low half, equal in the high half: 128 at most
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mine += (k[e] > prefix ? 1u : 0u) + (k[e] == prefix && k[e] != 0u ? 0x10000u : 0u);
+            uint32_t incl = mine;
+#pragma unroll
+            for (int s = 1; s < 32; s <<= 1) {
+                const uint32_t up = __shfl_up_sync(0xffffffffu, incl, s);
+                if (lane >= s) incl += up;
+            }
+            if (mine) {
+                uint32_t g = g0 + ((incl - mine) & 0xffffu), q = e0 + ((incl - mine) >> 16);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const bool above = k[e] > prefix, equal = k[e] == prefix && k[e] != 0u;
+                    if (above || (equal && q < left)) kept[g + min(q, left)] = lo + i + e;
+                    g += above, q += equal;
+                }
+            }
+            const uint32_t all = __shfl_sync(0xffffffffu, incl, 31);
+            g0 += all & 0xffffu;
+            e0 += all >> 16;
         }
-        g += __popc(bg & ((1u << lane) - 1u));
-        e += __popc(be & ((1u << lane) - 1u));
-        const int e_before = min(left, eq_done + e);
-        if (gt || (eq && eq_done + e < left)) {
-            const int at = done + g + (e_before - min(left, eq_done));
-            kept[at] = i;
-            wo[at] = p.w[b * p.w_sb + hk * p.w_sh + i];
-        }
-        done += gall + (min(left, eq_done + eall) - min(left, eq_done));
-        eq_done += eall;
-    }
-    for (int i = n_keep + tid; i < p.keep; i += 1024) kept[i] = -1, wo[i] = 0.f;
-    if (hk == 0 && tid == 0) p.new_lens[b] = n_keep;
+    for (int i = n_keep + rank * kEvictThreads + tid; i < p.keep; i += cluster * kEvictThreads) kept[i] = -1;
+    if (hk == 0 && rank == 0 && tid == 0) p.new_lens[b] = n_keep;
+    // no CTA leaves while another reads its counts
+    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
-// Kept row i of (b, hk) -> position i of the destination table's pages.
+// Kept row i of (b, hk) -> position i of the destination table's pages, K and V,
+// and its weight beside its position; 16 bytes to a thread and row, kGatherRows rows at once: that many copies on
+// their way are what the memory needs.
+constexpr int kGatherRows = 4;
+
 template <int ESIZE>
-__global__ void evict_gather_kernel(const EvictParams p) {
-    const int hk = blockIdx.y, b = blockIdx.z;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int c = (int)(i % p.chunks);
-    const int64_t to = i / p.chunks;
-    if (to >= p.keep) return;
-    const int from = p.kept[((int64_t)b * p.pool.Hkv + hk) * p.keep + to];
-    if (from < 0) return;
-    const int sp = page_of(p.src, p.pool.num_pages, b, from / p.pool.page);
-    const int dp = page_of(p.dst, p.pool.num_pages, b, (int)to / p.pool.page);
-    if (sp < 0 || dp < 0) return;
-    const int64_t ss = from % p.pool.page, ds = to % p.pool.page;
-    char *k = static_cast<char *>(p.pool.k), *v = static_cast<char *>(p.pool.v);
-    reinterpret_cast<int4 *>(k + (dp * p.pool.k_sp + hk * p.pool.k_sh + ds * p.pool.k_ss) * ESIZE)[c] =
-        reinterpret_cast<const int4 *>(k + (sp * p.pool.k_sp + hk * p.pool.k_sh + ss * p.pool.k_ss) * ESIZE)[c];
-    reinterpret_cast<int4 *>(v + (dp * p.pool.v_sp + hk * p.pool.v_sh + ds * p.pool.v_ss) * ESIZE)[c] =
-        reinterpret_cast<const int4 *>(v + (sp * p.pool.v_sp + hk * p.pool.v_sh + ss * p.pool.v_ss) * ESIZE)[c];
+__global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int hk = blockIdx.y, b = blockIdx.z, rows = 256 / p.chunks;  // rows of a pass of the block
+    const int c = threadIdx.x % p.chunks, r = threadIdx.x / p.chunks;
+    const int *kept = p.kept + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
+    const int weight_blocks = (p.keep + 1023) / 1024;
+    if ((int)blockIdx.x < weight_blocks) {  // the first blocks: 1024 weights each
+        const float *w = p.w + b * p.w_sb + hk * p.w_sh;
+        float *wo = p.w_out + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = blockIdx.x * 1024 + e * 256 + threadIdx.x;
+            if (i >= p.keep) break;
+            const int pos = kept[i];
+            wo[i] = pos >= 0 ? __ldg(w + pos) : 0.f;
+        }
+        return;
+    }
+    if (r >= rows) return;
+    const int64_t first = (int64_t)(blockIdx.x - weight_blocks) * rows * kGatherRows + r;
+    const char *k = static_cast<const char *>(p.pool.k) + hk * p.pool.k_sh * ESIZE + c * 16;
+    const char *v = static_cast<const char *>(p.pool.v) + hk * p.pool.v_sh * ESIZE + c * 16;
+    int from[kGatherRows], page[kGatherRows], to_page[kGatherRows];
+    int4 x[kGatherRows], y[kGatherRows];
+#pragma unroll
+    for (int e = 0; e < kGatherRows; ++e) from[e] = first + e * rows < p.keep ? kept[first + e * rows] : -1;
+#pragma unroll
+    for (int e = 0; e < kGatherRows; ++e) {
+        page[e] = to_page[e] = -1;
+        if (from[e] < 0) continue;
+        const uint32_t idx = p.pool.by_page.div(from[e]);
+        page[e] = page_of(p.src, p.pool.num_pages, b, (int)idx);
+        from[e] -= (int)idx * p.pool.page;
+        to_page[e] = page_of(p.dst, p.pool.num_pages, b, (int)p.pool.by_page.div((uint32_t)(first + e * rows)));
+    }
+#pragma unroll
+    for (int e = 0; e < kGatherRows; ++e)
+        if (page[e] >= 0) {
+            x[e] = *reinterpret_cast<const int4 *>(k + (page[e] * p.pool.k_sp + from[e] * p.pool.k_ss) * ESIZE);
+            y[e] = *reinterpret_cast<const int4 *>(v + (page[e] * p.pool.v_sp + from[e] * p.pool.v_ss) * ESIZE);
+        }
+#pragma unroll
+    for (int e = 0; e < kGatherRows; ++e)
+        if (page[e] >= 0 && to_page[e] >= 0) {
+            const int64_t to = first + e * rows;
+            const int64_t slot = to - (int64_t)p.pool.by_page.div((uint32_t)to) * p.pool.page;
+            *reinterpret_cast<int4 *>(const_cast<char *>(k) + (to_page[e] * p.pool.k_sp + slot * p.pool.k_ss) * ESIZE) = x[e];
+            *reinterpret_cast<int4 *>(const_cast<char *>(v) + (to_page[e] * p.pool.v_sp + slot * p.pool.v_ss) * ESIZE) = y[e];
+        }
 }
 
 }  // namespace gae

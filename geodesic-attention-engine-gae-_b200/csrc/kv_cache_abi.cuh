@@ -171,8 +171,11 @@ gae_status gae_paged_append(const gae_kv_pool *pool, const gae_paged_append_args
     p.chunks = (int)(pool->head_dim * es / 16);
     if (a->tokens > kMaxPositions) return fail(GAE_ERR_UNSUPPORTED, "more than 2^30 new tokens");
     p.tokens = (int)a->tokens;
-    const int64_t blocks = (a->tokens * p.chunks * pool->kv_heads + 255) / 256;
-    if (blocks > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many new rows");
+    p.by_chunks = gae::FastDiv::of((uint32_t)p.chunks);
+    p.by_heads = gae::FastDiv::of((uint32_t)p.pool.Hkv);
+    const int64_t pieces = a->tokens * p.chunks * pool->kv_heads, per_block = 256 * gae::kAppendRows;
+    if (pieces > INT32_MAX - per_block) return fail(GAE_ERR_UNSUPPORTED, "more than 2^31 pieces of new rows to a sequence");
+    const int64_t blocks = (pieces + per_block - 1) / per_block;
     const dim3 grid((unsigned)blocks, (unsigned)a->batch);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (es == 4) gae::paged_append_kernel<4><<<grid, 256, 0, st>>>(p);
@@ -355,13 +358,36 @@ gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *
     const int es = dtype_size(pool->dtype);
     p.chunks = (int)(pool->head_dim * es / 16);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    gae::evict_select_kernel<<<dim3((unsigned)pool->kv_heads, (unsigned)a->batch), 1024, 0, st>>>(p);
-    GAE_CUDA_TRY(cudaGetLastError());
-    const dim3 grid((unsigned)((a->keep * p.chunks + 255) / 256), (unsigned)pool->kv_heads, (unsigned)a->batch);
-    if (es == 4) gae::evict_gather_kernel<4><<<grid, 256, 0, st>>>(p);
-    else gae::evict_gather_kernel<2><<<grid, 256, 0, st>>>(p);
-    GAE_CUDA_TRY(cudaGetLastError());
-    return GAE_OK;
+    // As many CTAs to a row as the GPU has room for beside the other rows', each
+    // with 4096 positions at least; more where a CTA could not hold its keys.
+    const int64_t rows = a->batch * pool->kv_heads;
+    int cluster = 1;
+    while (cluster < gae::kEvictMaxCluster &&
+           ((int64_t)cluster * gae::kEvictMaxKeys < p.cap ||
+            ((int64_t)cluster * 4096 < p.cap && rows * cluster * 2 <= num_sms())))
+        cluster *= 2;
+    const int max_keys = (int)gae::min64(((p.cap + cluster - 1) / cluster + 3) / 4 * 4, gae::kEvictMaxKeys);
+    if (rows * cluster > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many rows");
+    const int smem = (2 * gae::kEvictBins + max_keys) * 4;
+    if ((s = set_smem(gae::evict_select_kernel, smem)) != GAE_OK) return s;
+    cudaLaunchConfig_t cfg;
+    memset(&cfg, 0, sizeof(cfg));
+    cfg.gridDim = dim3((unsigned)(rows * cluster));
+    cfg.blockDim = dim3(gae::kEvictThreads);
+    cfg.dynamicSmemBytes = (size_t)smem;
+    cfg.stream = st;
+    cudaLaunchAttribute at;
+    memset(&at, 0, sizeof(at));
+    at.id = cudaLaunchAttributeClusterDimension;
+    at.val.clusterDim.x = (unsigned)cluster;
+    at.val.clusterDim.y = at.val.clusterDim.z = 1;
+    cfg.attrs = &at;
+    cfg.numAttrs = 1;
+    GAE_CUDA_TRY(cudaLaunchKernelEx(&cfg, gae::evict_select_kernel, (const gae::EvictParams)p, cluster, max_keys));
+    const int64_t block_rows = 256 / p.chunks * gae::kGatherRows;
+    const dim3 grid((unsigned)((a->keep + block_rows - 1) / block_rows + (a->keep + 1023) / 1024), (unsigned)pool->kv_heads, (unsigned)a->batch);
+    return es == 4 ? launch_after(gae::evict_gather_kernel<4>, grid, 256, st, p)
+                   : launch_after(gae::evict_gather_kernel<2>, grid, 256, st, p);
 }
 
 }  // extern "C"
