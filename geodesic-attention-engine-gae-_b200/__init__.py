@@ -14,6 +14,8 @@ Device-tensor entry points (torch tensors on a CUDA device):
     quantize_rows_int8(x), attention_int8(...), int8_logits(...)
     paged_append, paged_attention, attention_key_weights, paged_evict: the
         paged key-value cache of single-token attention (kv_cache.py)
+    PagedKVCache, layer_stack_prefill, layer_stack_decode: a model's cache and
+        the GPT-2 stack over it, a prompt and then token by token
 Host drop-ins of the crate (numpy / sequences of float, fp32):
     waller_operator, waller_operator_parallel, standard_attention
 Scalar helpers of the crate (pure host logic, not the hot path):
@@ -715,6 +717,66 @@ class Gpt2Layer:
         return out
 
 
+    def _heads(self, qkv, *lead):
+        """q, k, v [*lead, heads, head_dim] as views of the packed projection."""
+        return qkv.view(*lead, 3, self.heads, self.d_model // self.heads).unbind(len(lead))
+
+    def _mlp(self, x1):
+        w = self.w
+        h = layernorm_rows(x1, w["ln2_gamma"], w["ln2_beta"], self.eps)
+        return linear(linear(h, w["w_fc"], w["b_fc"], gelu=True), w["w_fc2"], w["b_fc2"], res=x1)
+
+    def prefill(self, x, cache, layer):
+        """forward() of a prompt that also writes its keys and values (and, with a
+        budget, their weights) to layer `layer` of a PagedKVCache whose reserve()
+        has made room for it.  x: bf16 [B, S, d_model] contiguous, right-padded;
+        the cache's sequences have to be empty (a prompt attends to itself alone)."""
+        if any(cache.lengths):
+            raise GAEError(1, "prefill: the cache is not empty")
+        B, S, D = x.shape
+        w, x = self.w, x.reshape(B * S, D)
+        h = layernorm_rows(x, w["ln1_gamma"], w["ln1_beta"], self.eps)
+        q, k, v = (t.transpose(1, 2) for t in self._heads(linear(h, w["w_qkv"], w["b_qkv"]), B, S))
+        att, lse = attention(q, k, v, causal=True, return_lse=True)
+        cache.append(layer, k, v)
+        cache.add_prompt_weights(layer, q, k, lse)
+        att = att.transpose(1, 2).reshape(B * S, D)
+        return self._mlp(linear(att, w["w_proj"], w["b_proj"], res=x)).view(B, S, D)
+
+    def decode(self, x, cache, layer):
+        """One new token per sequence, x bf16 [B, d_model], over layer `layer` of
+        the cache, which takes in the token's key and value first."""
+        w = self.w
+        h = layernorm_rows(x, w["ln1_gamma"], w["ln1_beta"], self.eps)
+        q, k, v = self._heads(linear(h, w["w_qkv"], w["b_qkv"]), x.shape[0])
+        cache.append(layer, k.unsqueeze(2), v.unsqueeze(2))
+        att = cache.attend(layer, q).reshape(x.shape)
+        return self._mlp(linear(att, w["w_proj"], w["b_proj"], res=x))
+
+
+def layer_stack_prefill(layers, x, cache, counts=None):
+    """A prompt through `layers` into an empty PagedKVCache: x bf16 [B, S,
+    d_model], right-padded where counts (a list) says how many tokens each
+    sequence has.  Returns the hidden states [B, S, d_model]."""
+    if any(cache.lengths):
+        raise GAEError(1, "prefill: the cache is not empty")
+    cache.reserve(x.shape[1], counts)
+    for i, layer in enumerate(layers):
+        x = layer.prefill(x, cache, i)
+    cache.commit()
+    return x
+
+
+def layer_stack_decode(layers, x, cache):
+    """One new token per sequence through `layers`: x bf16 [B, d_model] to the
+    hidden states [B, d_model]."""
+    cache.reserve(1)
+    for i, layer in enumerate(layers):
+        x = layer.decode(x, cache, i)
+    cache.commit()
+    return x
+
+
 def layer_stack_forward(layers, x, out=None, workspace=None, stream=None):
     """Applies layers (a list of Gpt2Layer of one shape) in order through
     gae_layer_stack_fwd (one call, ping-pong buffers in the workspace)."""
@@ -881,6 +943,6 @@ def symphony_forward(x, k, v, w_up, w_down, norm1_w, norm2_w, tuning: TuningFork
 
 # ------------------------------------------------- paged key-value cache
 from .kv_cache import (KeyWeightsArgs, KvPool, PagedAppendArgs, PagedAttnArgs,  # noqa: E402
-                       PagedEvictArgs, attention_key_weights, paged_append, paged_attention,
+                       PagedEvictArgs, PagedKVCache, attention_key_weights, paged_append, paged_attention,
                        paged_evict)
 from .kv_cache import _bind as _kv_bind  # noqa: E402

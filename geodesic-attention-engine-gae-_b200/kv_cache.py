@@ -347,3 +347,134 @@ def paged_evict(k_pages, v_pages, page_table, seq_lens, weights, dst_table, *, k
 
     return _run(what, (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
                        ("seq_lens", seq_lens), ("weights", weights), ("dst_table", dst_table)), stream, body)
+
+
+class PagedKVCache:
+    """The keys and values of a batch of sequences for a model's layers.
+
+    Every sequence owns max_len positions' worth of pages; the layers share one
+    page table and one set of lengths.  A step over n new tokens is reserve(n),
+    then per layer append() and attend() (or, for a prompt, the whole-sequence
+    attention and add_prompt_weights()), then commit().  With a budget the cache
+    also keeps the weight that each key has drawn, and evict() brings sequences
+    longer than the budget back to it: the `recent` last positions and the
+    heaviest others, per layer and key head (spare pages of a budget's size are
+    held for that).
+
+    reserve, append, attend and commit launch on the current stream and may be
+    captured into a CUDA graph; `lengths`, the host's count that the capacity
+    check and evict() go by, does not move on a replay: refresh() reads it back
+    from the device."""
+
+    def __init__(self, n_layers, batch, kv_heads, head_dim, max_len, *, page_size=16, dtype=None, device="cuda",
+                 budget=None, recent=0):
+        torch = _torch()
+        if min(n_layers, batch, kv_heads, head_dim, max_len, page_size) < 1:
+            raise GAEError(1, "PagedKVCache: sizes must be positive")
+        if budget is not None and not 0 < budget <= max_len:
+            raise GAEError(1, f"PagedKVCache: budget must be in [1, {max_len}]")
+        if budget is not None and not 0 <= recent <= budget:
+            raise GAEError(1, "PagedKVCache: recent must be in [0, budget]")
+        dtype = torch.bfloat16 if dtype is None else dtype
+        self.batch, self.page_size, self.max_len, self.budget, self.recent = batch, page_size, max_len, budget, recent
+        per = -(-max_len // page_size)
+        spare = 0 if budget is None else -(-budget // page_size)
+        pages = batch * (per + spare)
+        shape = (pages, kv_heads, page_size, head_dim)
+        self.k = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        self.v = [torch.empty(shape, dtype=dtype, device=device) for _ in range(n_layers)]
+        ids = torch.arange(pages, dtype=torch.int32, device=device).view(batch, per + spare)
+        self.table = ids[:, :per].contiguous()
+        self.spare = ids[:, per:].contiguous() if spare else None
+        self.lens = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.next_lens = torch.zeros_like(self.lens)
+        self.weights = None if budget is None else [
+            torch.zeros((batch, kv_heads, per * page_size), dtype=torch.float32, device=device)
+            for _ in range(n_layers)]
+        self.lengths = [0] * batch
+        self._reserved = None
+
+    def reserve(self, tokens, counts=None):
+        """Makes room for `tokens` new tokens of every sequence (counts: a list
+        of how many of them each sequence really has)."""
+        n = [tokens] * self.batch if counts is None else [int(c) for c in counts]
+        if len(n) != self.batch or any(not 0 <= c <= tokens for c in n):
+            raise GAEError(1, f"PagedKVCache: counts must be {self.batch} numbers of [0, {tokens}]")
+        longest = max(a + b for a, b in zip(self.lengths, n))
+        if longest > self.max_len:
+            raise GAEError(1, f"PagedKVCache: {longest} positions, room for {self.max_len}")
+        torch = _torch()
+        self._reserved = n
+        if counts is None:
+            torch.add(self.lens, tokens, out=self.next_lens)
+        else:
+            torch.add(self.lens, torch.tensor(n, dtype=torch.int32, device=self.lens.device), out=self.next_lens)
+
+    def append(self, layer, k_new, v_new):
+        """Writes k_new/v_new [B, Hkv, T, D] behind the sequences of `layer`
+        (T as reserved; a sequence's tokens beyond its count are dropped)."""
+        if self._reserved is None:
+            raise GAEError(1, "PagedKVCache: append without reserve")
+        counts = None
+        if any(c != k_new.shape[2] for c in self._reserved):
+            counts = self.next_lens - self.lens
+        paged_append(k_new, v_new, self.k[layer], self.v[layer], self.table, self.lens, counts=counts)
+
+    def attend(self, layer, q, scale=None, out=None):
+        """Attention of one new token per sequence, q [B, H, D], over everything
+        appended so far; adds up the keys' weights where there is a budget."""
+        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.next_lens, scale=scale, out=out,
+                               weights=None if self.weights is None else self.weights[layer])
+
+    def add_prompt_weights(self, layer, q, k, lse, scale=None):
+        """Adds the weight that a prompt's queries put on its keys (an empty
+        cache's first tokens): q [B, H, T, D], k [B, Hkv, T, D] and the lse of
+        attention(q, k, v, causal=True, return_lse=True)."""
+        if self.weights is None:
+            return
+        if any(self.lengths):
+            raise GAEError(1, "PagedKVCache: prompt weights need an empty cache")
+        T = q.shape[2]
+        torch = _torch()
+        if any(c != T for c in self._reserved):  # queries beyond a sequence's own tokens weigh nothing
+            pad = torch.arange(T, device=lse.device)[None] >= self.next_lens[:, None]
+            lse = lse.masked_fill(pad[:, None], -math.inf)
+        attention_key_weights(q, k, lse, causal=True, scale=scale, out=self.weights[layer][:, :, :T], accumulate=True)
+
+    def commit(self):
+        """The reserved tokens become part of the sequences."""
+        if self._reserved is None:
+            raise GAEError(1, "PagedKVCache: commit without reserve")
+        self.lens.copy_(self.next_lens)
+        self.lengths = [a + b for a, b in zip(self.lengths, self._reserved)]
+        self._reserved = None
+
+    def refresh(self):
+        """Takes the host's lengths from the device (after replays; synchronises)."""
+        self.lengths = self.lens.tolist()
+
+    def evict(self):
+        """Brings every sequence back to the budget, if any is longer.  Returns
+        the kept positions per layer (int32 [B, Hkv, budget], -1 beyond the new
+        length), or None where there was nothing to do."""
+        if self.budget is None:
+            raise GAEError(1, "PagedKVCache: evict without a budget")
+        if self._reserved is not None:
+            raise GAEError(1, "PagedKVCache: evict between reserve and commit")
+        if max(self.lengths) <= self.budget:
+            return None
+        kept = []
+        for k, v, w in zip(self.k, self.v, self.weights):
+            lens, pos, left = paged_evict(k, v, self.table, self.lens, w, self.spare, keep=self.budget,
+                                          recent=self.recent)
+            w[:, :, : self.budget].copy_(left)
+            w[:, :, self.budget:].zero_()
+            kept.append(pos)
+        # The kept rows lie in the spare pages: they change places with the first ones.
+        n = self.spare.shape[1]
+        first = self.table[:, :n].clone()
+        self.table[:, :n].copy_(self.spare)
+        self.spare.copy_(first)
+        self.lens.copy_(lens)
+        self.lengths = [min(a, self.budget) for a in self.lengths]
+        return kept

@@ -187,3 +187,32 @@ def test_python_refusals(gae):
         with pytest.raises(gae.GAEError):
             call()
             pytest.fail(f"call {i} was accepted")
+
+
+def test_cache_refusals(gae):
+    """PagedKVCache's own bookkeeping, on CPU tensors: nothing is launched."""
+    new = lambda **kw: gae.PagedKVCache(1, 2, 2, 64, 40, page_size=16, device="cpu", **kw)  # noqa: E731
+    for bad in (dict(budget=0), dict(budget=41), dict(budget=8, recent=9)):
+        with pytest.raises(gae.GAEError):
+            new(**bad)
+    c = new()
+    assert c.table.shape == (2, 3) and c.table.unique().numel() == 6 and c.spare is None
+    k = torch.zeros(2, 2, 1, 64, dtype=torch.bfloat16)
+    for call in (lambda: c.append(0, k, k), c.commit, c.evict, lambda: c.reserve(41), lambda: c.reserve(3, [1]),
+                 lambda: c.reserve(3, [1, 4])):
+        with pytest.raises(gae.GAEError):
+            call()
+    c.reserve(30, [30, 7])
+    c.commit()
+    assert c.lengths == [30, 7] and c.lens.tolist() == [30, 7]
+    with pytest.raises(gae.GAEError):  # 30 + 11 > 40
+        c.reserve(11)
+    b = new(budget=20, recent=4)
+    assert b.spare.shape == (2, 2) and not set(b.spare.flatten().tolist()) & set(b.table.flatten().tolist())
+    b.reserve(20)
+    with pytest.raises(gae.GAEError):  # between reserve and commit
+        b.evict()
+    b.commit()
+    assert b.evict() is None
+    with pytest.raises(gae.GAEError):  # not empty any more
+        gae.layer_stack_prefill([], torch.zeros(2, 1, 128, dtype=torch.bfloat16), b)

@@ -473,3 +473,117 @@ def test_on_another_stream_and_captured(gae):
         ref = _evict_reference(k.cpu(), v.cpu(), table.cpu(), after.cpu(), w2.cpu(), dst.cpu(), 100, 8)
         assert torch.equal(n2.cpu(), ref[2]) and torch.equal(kept.cpu(), ref[3])
         assert torch.equal(k.cpu(), ref[0]) and torch.equal(v.cpu(), ref[1])
+
+
+# ------------------------------------------------------ a run of them together
+def _layers(gae, n, D, H, F):
+    """Weights larger than the usual 0.02, so that attention and its scores matter."""
+    layers = [gae.Gpt2Layer.random(D, H, F, seed=50 + i) for i in range(n)]
+    for layer in layers:
+        layer.w["w_qkv"].mul_(4)
+    return layers
+
+
+@pytest.mark.parametrize("D,H,page", [(256, 4, 16), (512, 4, 24)])
+def test_stack_decodes_what_it_computes_whole(gae, D, H, page):
+    """A prompt of ragged lengths, then token by token, against the stack over the whole sequence
+    (the layer tolerance of tests/test_layer_gpu.py: 2e-2 * max(1, |ref|))."""
+    B, S, steps, g = 3, 150, 9, _gen(30)
+    layers = _layers(gae, 2, D, H, 1024)
+    counts = [150, 33, 1]
+    x = torch.randn(B, S + steps, D, device="cuda", generator=g).bfloat16()
+    cache = gae.PagedKVCache(2, B, H, D // H, S + steps, page_size=page)
+    whole = [gae.layer_stack_forward(layers, x[b: b + 1, : counts[b] + steps].contiguous())[0].float() for b in range(B)]
+    close = lambda a, r: ((a.float() - r).abs() <= 2e-2 * r.abs().clamp(min=1)).all()  # noqa: E731
+    prompt = torch.zeros(B, S, D, device="cuda", dtype=torch.bfloat16)
+    for b, n in enumerate(counts):
+        prompt[b, :n] = x[b, :n]
+    y = gae.layer_stack_prefill(layers, prompt, cache, counts)
+    for b, n in enumerate(counts):
+        assert close(y[b, :n], whole[b][:n]), b
+    for t in range(steps):
+        y = gae.layer_stack_decode(layers, torch.stack([x[b, n + t] for b, n in enumerate(counts)]), cache)
+        for b, n in enumerate(counts):
+            assert close(y[b], whole[b][n + t]), (t, b)
+    torch.cuda.synchronize()
+    gae.device_status()
+    assert cache.lens.tolist() == cache.lengths == [n + steps for n in counts]
+    with pytest.raises(gae.GAEError):
+        gae.layer_stack_decode(layers, x[:, 0].contiguous(), cache)  # no room left
+
+
+def _dense(cache, layer):
+    """(key, value) lists per sequence in 64 bits, read through the cache's table."""
+    return [tuple(t.double().transpose(0, 1) for t in _rows(cache.k[layer], cache.v[layer], cache.table, b, n)[1:])
+            for b, n in enumerate(cache.lens.tolist())]
+
+
+def test_cache_within_a_budget(gae):
+    """Prompt, eviction, decoding past the budget and eviction again: the kept rows are those of the
+    heaviest keys, the weights are theirs, and decoding attends to exactly them."""
+    B, H, D, S, budget, recent, g = 2, 4, 256, 200, 64, 8, _gen(31)
+    layers = _layers(gae, 2, D, H, 512)
+    cache = gae.PagedKVCache(2, B, H, D // H, 256, page_size=16, budget=budget, recent=recent)
+    counts = [200, 90]
+    gae.layer_stack_prefill(layers, torch.randn(B, S, D, device="cuda", generator=g).bfloat16(), cache, counts)
+    for w in cache.weights:  # every real query hands out a weight of one per head (lse of 16-bit probabilities)
+        assert ((w.sum(-1) / torch.tensor(counts, device="cuda")[:, None] - 1).abs() <= 2.0 ** -7).all()
+        assert (w[1, :, 90:] == 0).all()
+    for turn in range(2):
+        before = [(_dense(cache, i), cache.weights[i].clone()) for i in range(2)]
+        was = list(cache.lengths)
+        kept = cache.evict()
+        assert cache.lengths == [min(n, budget) for n in was] == cache.lens.tolist()
+        for i in range(2):
+            rows, w = before[i]
+            after = _dense(cache, i)
+            for b, n in enumerate(was):
+                m = min(n, budget)
+                for h in range(H):
+                    x = w[b, h, :n].clone()
+                    x[n - recent:] = math.inf
+                    want = torch.sort(x, descending=True, stable=True).indices[:m].sort().values
+                    assert torch.equal(kept[i][b, h, :m].long(), want)
+                    assert torch.equal(after[b][0][h], rows[b][0][h][want])
+                    assert torch.equal(after[b][1][h], rows[b][1][h][want])
+                    assert torch.equal(cache.weights[i][b, h, :m], w[b, h, want])
+        for _ in range(10):
+            gae.layer_stack_decode(layers, torch.randn(B, D, device="cuda", generator=g).bfloat16(), cache)
+        assert cache.lengths == [budget + 10] * B
+        # one more token by hand: attention over what the cache now holds
+        q = torch.randn(B, H, D // H, device="cuda", generator=g).bfloat16()
+        w = cache.weights[1].clone()
+        cache.next_lens.copy_(cache.lens)
+        out = cache.attend(1, q)
+        for b in range(B):
+            k, v = _dense(cache, 1)[b]
+            p = torch.softmax(torch.einsum("hd,hnd->hn", q[b].double(), k) / math.sqrt(D // H), -1)
+            assert ((out[b].double() - torch.einsum("hn,hnd->hd", p, v)).abs() <= 2.0 ** -8 * v.abs().max()).all()
+            assert ((cache.weights[1][b, :, : budget + 10] - w[b, :, : budget + 10] - p).abs() <= 1e-4).all()
+
+
+def test_decoding_step_in_a_graph(gae):
+    """A captured decoding step replayed token by token gives what the eager steps give."""
+    B, H, D, steps, g = 2, 4, 256, 20, _gen(32)
+    layers = _layers(gae, 2, D, H, 512)
+    x = torch.randn(steps, B, D, device="cuda", generator=g).bfloat16()
+    eager, graphed = (gae.PagedKVCache(2, B, H, D // H, 64, budget=64) for _ in range(2))
+    want = [gae.layer_stack_decode(layers, x[t], eager) for t in range(steps)]
+    xin = x[0].clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        gae.layer_stack_decode(layers, xin, graphed)  # token 0, and the warm-up
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = gae.layer_stack_decode(layers, xin, graphed)
+    for t in range(1, steps):
+        xin.copy_(x[t])
+        graph.replay()
+        assert torch.equal(y, want[t]), t
+    for a, b in zip(eager.weights, graphed.weights):
+        assert torch.equal(a, b)
+    assert graphed.lengths != [steps] * B  # the host has not seen the replays
+    graphed.refresh()
+    assert graphed.lengths == graphed.lens.tolist() == [steps] * B
