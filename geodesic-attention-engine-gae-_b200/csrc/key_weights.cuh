@@ -221,10 +221,12 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
         const int g = warp >> 2, key = (warp & 3) * 32 + lane;
         const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 128;
         const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
-        // Columns before this are queries before this thread's (this warp's last)
-        // key, for the first query tile; beyond it every tile moves it by 128.
-        const int64_t first = p.causal ? (int64_t)j * 128 + key - p.off : INT64_MIN / 2;
-        const int64_t first_warp = first + 31 - lane;
+        // Query rows before this are before this thread's key (this warp's lowest,
+        // its highest): all an epilogue has to know of the mask, within [0, Nq].
+        auto first_row = [&](int k) {
+            return p.causal ? (int)max64(0, min64(p.Nq, (int64_t)j * 128 + k - p.off)) : 0;
+        };
+        const int first = first_row(key), first_low = first_row(key - lane), first_high = first_row(key - lane + 31);
         if (g == 1) next_tile();
         for (int it = g; it < n_it; it += 2) {
             const int q0 = (i0 + i) * 128;
@@ -234,21 +236,16 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             tc_fence_after();
             const uint32_t sl = base + Cfg::kOffLse + (it & 3) * 512;
             uint64_t acc[4] = {};
-            // a warp whose every key is seen by all 128 queries needs no mask
-            const bool full = first_warp <= q0 && q0 + 128 <= p.Nq;
-            // columns [lo, hi) count; those from hi on are no queries (their rows
-            // are zeros: a NaN key would reach the sum)
-            const int lo = (int)max64(0, min64(128, first - q0)), hi = min(128, p.Nq - q0);
+            if (first_high <= q0 && q0 + 128 <= p.Nq) {  // every key of the warp is seen by all 128 queries
 #pragma unroll
-            for (int c0 = 0; c0 < 128; c0 += 32) {
-                uint32_t r[32];
-                tmem_ld32(tS + c0, r);
-                tmem_wait_ld();
-                if (c0 == 96) {
-                    tc_fence_before();
-                    mbar_arrive(bar_s_empty(g));
-                }
-                if (full) {
+                for (int c0 = 0; c0 < 128; c0 += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(tS + c0, r);
+                    tmem_wait_ld();
+                    if (c0 == 96) {
+                        tc_fence_before();
+                        mbar_arrive(bar_s_empty(g));
+                    }
 #pragma unroll
                     for (int e = 0; e < 16; e += 2) {
                         uint64_t n[2];
@@ -269,7 +266,17 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
                             acc[(e + u) & 3] = f2_add(acc[(e + u) & 3], w);
                         }
                     }
-                } else {
+                }
+            } else {
+                // Columns [lo, hi) count; those from hi on are no queries (their rows
+                // are zeros: a NaN key would reach the sum).  32 columns that no key
+                // of the warp counts are passed over.
+                const int lo = first - q0, hi = min(128, p.Nq - q0);
+#pragma unroll 1
+                for (int c0 = max(0, first_low - q0) & ~31; c0 < hi; c0 += 32) {
+                    uint32_t r[32];
+                    tmem_ld32(tS + c0, r);
+                    tmem_wait_ld();
 #pragma unroll
                     for (int e = 0; e < 16; ++e) {
                         uint64_t n0;
@@ -282,6 +289,8 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
                         acc[e & 3] = f2_add(acc[e & 3], f2_pack(w0, w1));
                     }
                 }
+                tc_fence_before();
+                mbar_arrive(bar_s_empty(g));
             }
             // a tile's sum first, then the total: the longest chains stay short
             float a, c;
