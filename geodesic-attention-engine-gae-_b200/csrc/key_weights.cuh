@@ -9,11 +9,12 @@
 // The scores are computed transposed, keys as the 128 rows of a tcgen05 tile
 // and queries as its columns: a TMEM lane is then one key, so a thread adds up
 // its key's weights in registers and no two threads ever share a sum (no
-// atomics, the same bits every time).  One CTA per (128-key tile, key head,
-// batch): K stays in shared memory, the tiles of 128 queries of all the head's
-// query heads stream through a TMA ring, two S tiles alternate in TMEM, each
-// with a warpgroup of its own that exponentiates it while the other's product runs.  Two CTAs to
-// an SM.
+// atomics, the same bits every time).  One CTA per (two 128-key tiles, key head,
+// batch), two CTAs to an SM: K stays in shared memory, the tiles of 128 queries
+// of all the head's query heads stream through TMA, and each key tile has an S
+// tile in TMEM and a warpgroup that exponentiates it while the other three
+// tiles' products and exponentials run.  One key tile to a CTA read every query
+// tile from L2 twice as often and was bound by that, at 6.2 TB/s.
 //
 // What bounds it: one exponential per score.  The MUFU gives 16 a cycle and
 // SM, a 128 x 128 tile takes it 1024 cycles where the products at head_dim 128
@@ -42,7 +43,7 @@ enum KeyWeightsWaitSite : unsigned {
 };
 
 #ifndef GAE_KW_POLY_PERIOD
-#define GAE_KW_POLY_PERIOD 4
+#define GAE_KW_POLY_PERIOD 3
 #endif
 constexpr int kKwPolyPeriod = GAE_KW_POLY_PERIOD;
 
@@ -77,10 +78,9 @@ __device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
 template <int D>
 struct KeyWeightsCfg {
     static constexpr int kBox = 128 * 128, kPanels = D * 2 / 128, kTile = kPanels * kBox;
-    static constexpr int kStages = D == 128 ? 2 : 4;
-    static constexpr int kOffK = 0, kOffQ = kTile, kOffLse = kOffQ + kStages * kTile;  // lse: 4 tiles of 128
-    static constexpr int kOffRed = kOffLse + 4 * 128 * 4;                               // 128 sums of the second warpgroup
-    static constexpr int kOffBar = kOffRed + 128 * 4;
+    static constexpr int kStages = D == 128 ? 1 : 3;
+    static constexpr int kOffK = 0, kOffQ = 2 * kTile, kOffLse = kOffQ + kStages * kTile;  // lse: 2 tiles of 128
+    static constexpr int kOffBar = kOffLse + 2 * 128 * 4;
     static constexpr int kNumBars = 2 + 2 * kStages + 4;  // k, done, q_full/q_empty, s_full/s_empty [2]
     static constexpr int kPayload = kOffBar + kNumBars * 8 + 16;
     static constexpr int kSmem = kPayload + 1024;  // slack for the 1024-byte alignment of the swizzle atoms
@@ -102,27 +102,28 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
     }
     const uint32_t sK = base + Cfg::kOffK, sBar = base + Cfg::kOffBar;
     auto sQ = [&](int st) { return base + Cfg::kOffQ + st * Cfg::kTile; };
-    float *s_lse = reinterpret_cast<float *>(smem + Cfg::kOffLse), *s_red = reinterpret_cast<float *>(smem + Cfg::kOffRed);
+    float *s_lse = reinterpret_cast<float *>(smem + Cfg::kOffLse);
     const uint32_t bar_k = sBar, bar_done = sBar + 8;
     auto bar_q_full = [&](int st) { return sBar + 8u * (2 + st); };
     auto bar_q_empty = [&](int st) { return sBar + 8u * (2 + Cfg::kStages + st); };
-    auto bar_s_full = [&](int bf) { return sBar + 8u * (2 + 2 * Cfg::kStages + bf); };
-    auto bar_s_empty = [&](int bf) { return sBar + 8u * (4 + 2 * Cfg::kStages + bf); };
+    auto bar_s_full = [&](int kt) { return sBar + 8u * (2 + 2 * Cfg::kStages + kt); };
+    auto bar_s_empty = [&](int kt) { return sBar + 8u * (4 + 2 * Cfg::kStages + kt); };
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::kOffBar + Cfg::kNumBars * 8);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int no_abort = 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-    // Key tiles in ascending order: under a causal mask the first have the most queries.
+    // Pairs of key tiles in ascending order: under a causal mask the first have the most queries.
     const int rows = p.B * p.Hkv;
     const int j = blockIdx.x / rows, b = blockIdx.x % rows / p.Hkv, hk = blockIdx.x % rows % p.Hkv, split = blockIdx.y;
     const int G = p.H / p.Hkv, nq = (p.Nq + 127) / 128;
-    int i0 = 0;  // first query tile that sees a key of this tile
-    if (p.causal) i0 = (int)min64(nq, max64(0, (int64_t)j * 128 - p.off) / 128);
+    const int n_kt = (int64_t)j * 256 + 128 < p.Nkv ? 2 : 1;  // key tiles that exist
+    int i0 = 0;  // first query tile that sees a key of this pair
+    if (p.causal) i0 = (int)min64(nq, max64(0, (int64_t)j * 256 - p.off) / 128);
     const int per_head = nq - i0, all = per_head * G;
     const int t0 = (int)((int64_t)all * split / p.splits), t1 = (int)((int64_t)all * (split + 1) / p.splits);
     const int n_it = t1 - t0;
-    // The query tile at hand: head h, tile i of those that see this key tile.
+    // The query tile at hand: head h, tile i of those that see these keys.
     int h = hk * G, i = 0;
     if (n_it > 0) h += t0 / per_head, i = t0 % per_head;
     auto next_tile = [&] {
@@ -136,9 +137,9 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             mbar_init(bar_q_full(st), 1);
             mbar_init(bar_q_empty(st), 1);
         }
-        for (int bf = 0; bf < 2; ++bf) {
-            mbar_init(bar_s_full(bf), 1 + 32);  // the products, and the lanes of the lse warp
-            mbar_init(bar_s_empty(bf), 128);
+        for (int kt = 0; kt < 2; ++kt) {
+            mbar_init(bar_s_full(kt), 1 + 32);  // the products, and the lanes of the lse warp
+            mbar_init(bar_s_empty(kt), 128);
         }
         *abort_flag = 0;
         fence_mbar_init();
@@ -152,13 +153,13 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
     tc_fence_after();
     const uint32_t tmem = *tmem_slot;
 
-    float total = 0.f;
     if (warp == Cfg::kTmaWarp) {
         if (lane == 0 && n_it > 0) {
             tma_prefetch_desc(&p.tm_q);
-            mbar_expect_tx(bar_k, Cfg::kTile);
-            for (int hf = 0; hf < Cfg::kPanels; ++hf)
-                tma_load_4d(sK + hf * Cfg::kBox, &p.tm_k, bar_k, hf * 64, j * 128, hk, b);
+            mbar_expect_tx(bar_k, n_kt * Cfg::kTile);
+            for (int kt = 0; kt < n_kt; ++kt)
+                for (int hf = 0; hf < Cfg::kPanels; ++hf)
+                    tma_load_4d(sK + kt * Cfg::kTile + hf * Cfg::kBox, &p.tm_k, bar_k, hf * 64, j * 256 + kt * 128, hk, b);
             int it = 0;
             for (; it < n_it; ++it) {
                 const int st = it % Cfg::kStages, use = it / Cfg::kStages;
@@ -178,26 +179,28 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             constexpr uint32_t id = idesc_f16(128, 128, kBF16, false, false);
             bool ok = mbar_wait(bar_k, 0, kSiteKwK, abort_flag);
             for (int it = 0; it < n_it && ok; ++it) {
-                const int st = it % Cfg::kStages, bf = it & 1;
-                if (it >= 2 && !(ok = mbar_wait(bar_s_empty(bf), ((it >> 1) - 1) & 1, kSiteKwSEmpty, abort_flag))) break;
+                const int st = it % Cfg::kStages;
                 if (!(ok = mbar_wait(bar_q_full(st), (it / Cfg::kStages) & 1, kSiteKwQFull, abort_flag))) break;
-                tc_fence_after();
+                for (int kt = 0; kt < n_kt; ++kt) {
+                    if (it > 0 && !(ok = mbar_wait(bar_s_empty(kt), (it - 1) & 1, kSiteKwSEmpty, abort_flag))) break;
+                    tc_fence_after();
 #pragma unroll
-                for (int kk = 0; kk < D / 16; ++kk) {
-                    const uint32_t o = (kk >> 2) * Cfg::kBox + (kk & 3) * 32;
-                    umma_f16_ss(tmem + bf * 128, smem_desc_sw128(sK + o, 16, 1024), smem_desc_sw128(sQ(st) + o, 16, 1024),
-                                id, kk > 0);
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint32_t o = (kk >> 2) * Cfg::kBox + (kk & 3) * 32;
+                        umma_f16_ss(tmem + kt * 128, smem_desc_sw128(sK + kt * Cfg::kTile + o, 16, 1024),
+                                    smem_desc_sw128(sQ(st) + o, 16, 1024), id, kk > 0);
+                    }
+                    umma_commit(bar_s_full(kt));
                 }
                 umma_commit(bar_q_empty(st));
-                umma_commit(bar_s_full(bf));
             }
             umma_commit(bar_done);
             mbar_wait(bar_done, 0, kSiteKwDone, &no_abort);
         }
     } else if (warp == Cfg::kLseWarp) {
-        // -lse of the tile's queries in log2; -inf where the row saw no key.  Four
-        // buffers: the warpgroup that has let go of S tile it - 2 is done with
-        // tile it - 4.
+        // -lse of the tile's queries in log2; -inf where the row saw no key.  Two
+        // buffers: warpgroups that have let go of S tile it - 1 are done with tile
+        // it - 2.
         auto fetch = [&](float (&v)[4]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -210,31 +213,33 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
         float v[4];
         if (n_it > 0) fetch(v);
         for (int it = 0; it < n_it; ++it) {
-            if (it >= 2 && !mbar_wait(bar_s_empty(it & 1), ((it >> 1) - 1) & 1, kSiteKwSEmpty, abort_flag)) break;
+            bool ok = true;
+            for (int kt = 0; kt < n_kt && it > 0; ++kt)
+                ok = ok && mbar_wait(bar_s_empty(kt), (it - 1) & 1, kSiteKwSEmpty, abort_flag);
+            if (!ok) break;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s_lse[(it & 3) * 128 + e * 32 + lane] = v[e];
+            for (int e = 0; e < 4; ++e) s_lse[(it & 1) * 128 + e * 32 + lane] = v[e];
             if (it + 1 < n_it) fetch(v);
-            mbar_arrive(bar_s_full(it & 1));
+            for (int kt = 0; kt < n_kt; ++kt) mbar_arrive(bar_s_full(kt));
         }
     } else {
-        // -------------- epilogue: warpgroup g takes every second S tile, thread = key
+        // ------------------------ epilogue: warpgroup g has key tile g, thread = key
         const int g = warp >> 2, key = (warp & 3) * 32 + lane;
         const uint32_t tS = tmem + ((uint32_t)((warp & 3) * 32) << 16) + g * 128;
         const uint64_t sl2 = f2_pack(p.scale_log2, p.scale_log2);
+        float total = 0.f;
         // Query rows before this are before this thread's key (this warp's lowest,
         // its highest): all an epilogue has to know of the mask, within [0, Nq].
         auto first_row = [&](int k) {
-            return p.causal ? (int)max64(0, min64(p.Nq, (int64_t)j * 128 + k - p.off)) : 0;
+            return p.causal ? (int)max64(0, min64(p.Nq, (int64_t)j * 256 + g * 128 + k - p.off)) : 0;
         };
         const int first = first_row(key), first_low = first_row(key - lane), first_high = first_row(key - lane + 31);
-        if (g == 1) next_tile();
-        for (int it = g; it < n_it; it += 2) {
+        for (int it = 0; it < n_it && g < n_kt; ++it) {
             const int q0 = (i0 + i) * 128;
             next_tile();
-            next_tile();
-            if (!mbar_wait(bar_s_full(g), (it >> 1) & 1, kSiteKwS, abort_flag)) break;
+            if (!mbar_wait(bar_s_full(g), it & 1, kSiteKwS, abort_flag)) break;
             tc_fence_after();
-            const uint32_t sl = base + Cfg::kOffLse + (it & 3) * 512;
+            const uint32_t sl = base + Cfg::kOffLse + (it & 1) * 512;
             uint64_t acc[4] = {};
             if (first_high <= q0 && q0 + 128 <= p.Nq) {  // every key of the warp is seen by all 128 queries
 #pragma unroll
@@ -297,22 +302,17 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             f2_unpack(f2_add(f2_add(acc[0], acc[1]), f2_add(acc[2], acc[3])), a, c);
             total += a + c;
         }
-        if (g == 1) s_red[key] = total;
-    }
-    __syncthreads();
-    if (warp < 4) {
-        const int key = warp * 32 + lane;
-        const int64_t c = (int64_t)j * 128 + key;
+        const int64_t c = (int64_t)j * 256 + g * 128 + key;
         if (c < p.Nkv) {
-            const float w = total + s_red[key];
             if (p.part) {
-                p.out[split * p.part + ((int64_t)b * p.Hkv + hk) * p.Nkv + c] = w;
+                p.out[split * p.part + ((int64_t)b * p.Hkv + hk) * p.Nkv + c] = total;
             } else {
                 float *o = p.out + b * p.o_sb + hk * p.o_sh + c;
-                *o = p.accumulate ? *o + w : w;
+                *o = p.accumulate ? *o + total : total;
             }
         }
     }
+    __syncthreads();
     if (warp == Cfg::kMmaWarp) {
         tc_fence_after();
         tmem_dealloc(tmem, Cfg::kTmemCols);

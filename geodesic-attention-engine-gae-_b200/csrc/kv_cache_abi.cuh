@@ -74,11 +74,11 @@ PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool
     return w;
 }
 
-// How many CTAs share a key tile's queries.  One where the key tiles fill the
+// How many CTAs share a pair of key tiles' queries.  One where the pairs fill the
 // GPU (two CTAs to an SM); else enough to fill it, as long as each is left with
 // 4 query tiles.
 int key_weights_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nkv) {
-    const int64_t units = B * Hkv * ((Nkv + 127) / 128), tiles = H / Hkv * ((Nq + 127) / 128);
+    const int64_t units = B * Hkv * ((Nkv + 255) / 256), tiles = H / Hkv * ((Nq + 127) / 128);
     const int64_t want = (2 * num_sms() + units - 1) / units;
     return (int)gae::max64(1, gae::min64(want, tiles / 4));
 }
@@ -315,7 +315,7 @@ gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
     p.splits = key_weights_splits(a->batch, a->heads, a->kv_heads, a->seq_q, a->seq_kv);
     p.part = p.splits > 1 ? a->batch * a->kv_heads * a->seq_kv : 0;
     p.out = p.splits > 1 ? static_cast<float *>(a->workspace) : a->out;
-    const int64_t units = a->batch * a->kv_heads * ((a->seq_kv + 127) / 128);
+    const int64_t units = a->batch * a->kv_heads * ((a->seq_kv + 255) / 256);
     if (units > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many key tiles");
     const dim3 grid((unsigned)units, (unsigned)p.splits);
     if (D == 128) s = bf16 ? launch_key_weights<128, true>(p, grid, st) : launch_key_weights<128, false>(p, grid, st);
