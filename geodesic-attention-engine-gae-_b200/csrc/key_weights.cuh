@@ -112,6 +112,7 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int no_abort = 0;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
     // Pairs of key tiles in ascending order: under a causal mask the first have the most queries.
     const int rows = p.B * p.Hkv;
@@ -322,9 +323,11 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
 // Adds the splits' parts in their order.
 __global__ void key_weights_sum_kernel(const float *parts, float *out, int64_t o_sb, int64_t o_sh, int Hkv, int Nkv,
                                        int64_t part, int splits, int accumulate) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= part) return;
     float w = 0.f;
+#pragma unroll 4
     for (int s = 0; s < splits; ++s) w += parts[s * part + i];
     const int64_t row = i / Nkv;
     float *o = out + row / Hkv * o_sb + row % Hkv * o_sh + i % Nkv;

@@ -74,13 +74,13 @@ PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool
     return w;
 }
 
-// How many CTAs share a pair of key tiles' queries.  One where the pairs fill the
-// GPU (two CTAs to an SM); else enough to fill it, as long as each is left with
-// 4 query tiles.
+// How many CTAs share a pair of key tiles' queries: enough to fill the GPU (two
+// CTAs to an SM) as long as each is left with 4 query tiles.  (Four times as
+// many, so that a causal mask's long units end together, gained nothing: 178
+// against 180 us at 8192 x 8192, 16 heads.)
 int key_weights_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nkv) {
     const int64_t units = B * Hkv * ((Nkv + 255) / 256), tiles = H / Hkv * ((Nq + 127) / 128);
-    const int64_t want = (2 * num_sms() + units - 1) / units;
-    return (int)gae::max64(1, gae::min64(want, tiles / 4));
+    return (int)gae::max64(1, gae::min64((2 * num_sms() + units - 1) / units, tiles / 4));
 }
 
 template <int D, bool kBF16>
@@ -322,10 +322,8 @@ gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
     else s = bf16 ? launch_key_weights<64, true>(p, grid, st) : launch_key_weights<64, false>(p, grid, st);
     if (s != GAE_OK || p.splits == 1) return s;
     const int64_t blocks = (p.part + 255) / 256;
-    gae::key_weights_sum_kernel<<<(unsigned)blocks, 256, 0, st>>>(p.out, a->out, p.o_sb, p.o_sh, p.Hkv, p.Nkv, p.part,
-                                                                  p.splits, p.accumulate);
-    GAE_CUDA_TRY(cudaGetLastError());
-    return GAE_OK;
+    return launch_after(gae::key_weights_sum_kernel, dim3((unsigned)blocks), 256, st, (const float *)p.out, a->out, p.o_sb,
+                        p.o_sh, p.Hkv, p.Nkv, p.part, p.splits, p.accumulate);
 }
 
 gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *a, void *stream) {
