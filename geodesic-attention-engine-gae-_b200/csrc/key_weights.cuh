@@ -42,10 +42,7 @@ enum KeyWeightsWaitSite : unsigned {
     kSiteKwDone = 0x506, kSiteKwSmem = 0x507,
 };
 
-#ifndef GAE_KW_POLY_PERIOD
-#define GAE_KW_POLY_PERIOD 3
-#endif
-constexpr int kKwPolyPeriod = GAE_KW_POLY_PERIOD;
+constexpr int kKwPolyPeriod = 3;
 
 // 2^x for a pair of x <= 2^22 on the FMA pipe: exp2_poly_x2's range reduction
 // with a polynomial of degree 5, whose coefficients are the minimax fit of 2^f

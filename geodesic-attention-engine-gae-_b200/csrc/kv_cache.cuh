@@ -142,10 +142,7 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 // and stay in shared memory (positions beyond kMaxKeys are formed again), only
 // histograms and counts cross the cluster.  What bounds it is latency: one
 // barrier of the cluster to a digit.
-#ifndef GAE_EV_THREADS
-#define GAE_EV_THREADS 1024
-#endif
-constexpr int kEvictThreads = GAE_EV_THREADS, kEvictWarps = kEvictThreads / 32, kEvictBins = 2048;
+constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32, kEvictBins = 2048;
 constexpr int kEvictMaxCluster = 8, kEvictMaxKeys = 40960;
 
 // A cluster barrier after which the CTAs see what the others wrote before it:

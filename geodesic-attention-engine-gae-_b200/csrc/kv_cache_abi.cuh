@@ -2,15 +2,19 @@
 // weights: argument checks and launches.  Included by gae_abi.cu after its
 // helpers (fail, set_smem, num_sms): one translation unit.
 #pragma once
+#include <initializer_list>
 
 namespace {
 
 int dtype_size(gae_dtype t) { return t == GAE_DTYPE_F32 ? 4 : t == GAE_DTYPE_BF16 || t == GAE_DTYPE_F16 ? 2 : 0; }
 
-// Strides that keep every row on a 16-byte boundary.
-bool row_strides(const int64_t *s, int n, int esize) {
-    for (int i = 0; i < n; ++i)
-        if (s[i] < 0 || (s[i] * esize) % 16) return false;
+// Strides that keep every row on a 16-byte boundary; what stands for a
+// dimension of one element is never used.
+bool row_strides(const int64_t *s, std::initializer_list<int64_t> sizes, int esize) {
+    for (int64_t n : sizes) {
+        if (n > 1 && (*s < 0 || (*s * esize) % 16)) return false;
+        ++s;
+    }
     return true;
 }
 
@@ -31,7 +35,8 @@ gae_status check_pool(const gae_kv_pool *pl, gae::KvPool *out) {
                     (long long)pl->head_dim);
     if (pl->num_pages > 0 && (!pl->k || !pl->v)) return fail(GAE_ERR_INVALID_ARG, "pool pointers are NULL");
     if (!aligned16(pl->k) || !aligned16(pl->v)) return fail(GAE_ERR_INVALID_ARG, "pools must be 16-byte aligned");
-    if (!row_strides(pl->k_stride, 3, es) || !row_strides(pl->v_stride, 3, es))
+    if (!row_strides(pl->k_stride, {pl->num_pages, pl->kv_heads, pl->page_size}, es) ||
+        !row_strides(pl->v_stride, {pl->num_pages, pl->kv_heads, pl->page_size}, es))
         return fail(GAE_ERR_INVALID_ARG, "pool strides must be non-negative multiples of 16 bytes");
     out->k = pl->k; out->v = pl->v;
     out->k_sp = pl->k_stride[0]; out->k_sh = pl->k_stride[1]; out->k_ss = pl->k_stride[2];
@@ -45,7 +50,7 @@ gae_status check_pool(const gae_kv_pool *pl, gae::KvPool *out) {
 gae_status check_table(const int32_t *entry, int64_t stride, int64_t max_pages, int64_t batch, int64_t page,
                        gae::PageTable *out) {
     if (max_pages < 0 || stride < 0) return fail(GAE_ERR_INVALID_ARG, "negative page table size or stride");
-    if (max_pages > 0 && !entry) return fail(GAE_ERR_INVALID_ARG, "page table is NULL");
+    if (max_pages > 0 && batch > 0 && !entry) return fail(GAE_ERR_INVALID_ARG, "page table is NULL");
     if (max_pages > kMaxPositions / page)
         return fail(GAE_ERR_UNSUPPORTED, "a page table of more than 2^30 positions");
     out->entry = entry; out->stride = stride; out->max_pages = (int)max_pages;
@@ -160,8 +165,9 @@ gae_status gae_paged_append(const gae_kv_pool *pool, const gae_paged_append_args
     if (a->batch == 0 || a->tokens == 0) return GAE_OK;
     const int es = dtype_size(pool->dtype);
     if (!a->k_new || !a->v_new || !a->start) return fail(GAE_ERR_INVALID_ARG, "NULL pointer in append arguments");
-    if (!aligned16(a->k_new) || !aligned16(a->v_new) || !row_strides(a->k_new_stride, 3, es) ||
-        !row_strides(a->v_new_stride, 3, es))
+    if (!aligned16(a->k_new) || !aligned16(a->v_new) ||
+        !row_strides(a->k_new_stride, {a->batch, pool->kv_heads, a->tokens}, es) ||
+        !row_strides(a->v_new_stride, {a->batch, pool->kv_heads, a->tokens}, es))
         return fail(GAE_ERR_INVALID_ARG, "new rows must be 16-byte aligned, with non-negative strides of 16 bytes");
     if (a->batch > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch > 65535");
     p.k_new = a->k_new; p.v_new = a->v_new;
@@ -207,11 +213,16 @@ gae_status gae_paged_attn_fwd(const gae_kv_pool *pool, const gae_paged_attn_args
         return fail(GAE_ERR_UNSUPPORTED, "batch or heads > 65535, or more than 2^31 - 1 rows");
     const int es = dtype_size(pool->dtype);
     if (!a->q || !a->o || !a->seq_lens) return fail(GAE_ERR_INVALID_ARG, "NULL pointer in paged attention arguments");
-    if (!aligned16(a->q) || !aligned16(a->o) || !row_strides(a->q_stride, 2, es) || !row_strides(a->o_stride, 2, es))
+    if (!aligned16(a->q) || !aligned16(a->o) || !row_strides(a->q_stride, {a->batch, a->heads}, es) ||
+        !row_strides(a->o_stride, {a->batch, a->heads}, es))
         return fail(GAE_ERR_INVALID_ARG, "q and o must be 16-byte aligned, with non-negative strides of 16 bytes");
     if (!(a->scale >= 0.f)) return fail(GAE_ERR_UNSUPPORTED, "negative or NaN scale");
     if ((a->weights != nullptr) != (a->weights_out != nullptr))
         return fail(GAE_ERR_INVALID_ARG, "weights and weights_out go together");
+    // Rows that lie on one another cannot be written.
+    if ((a->batch > 1 && a->o_stride[0] == 0) || (a->heads > 1 && a->o_stride[1] == 0) ||
+        (a->weights_out && ((a->batch > 1 && a->w_out_stride[0] == 0) || (pool->kv_heads > 1 && a->w_out_stride[1] == 0))))
+        return fail(GAE_ERR_INVALID_ARG, "output stride of 0");
     if (a->weights_out && (a->w_stride[0] < 0 || a->w_stride[1] < 0 || a->w_out_stride[0] < 0 || a->w_out_stride[1] < 0))
         return fail(GAE_ERR_INVALID_ARG, "negative weights stride");
     const int64_t cap = a->max_pages * pool->page_size;
@@ -272,11 +283,14 @@ gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
     if (a->seq_kv == 0) return GAE_OK;
     if (!a->out || (a->seq_q > 0 && (!a->q || !a->k || !a->lse)))
         return fail(GAE_ERR_INVALID_ARG, "NULL pointer in key weights arguments");
-    if (!aligned16(a->q) || !aligned16(a->k) || !row_strides(a->q_stride, 3, 2) || !row_strides(a->k_stride, 3, 2))
+    if (!aligned16(a->q) || !aligned16(a->k) || !row_strides(a->q_stride, {a->batch, a->heads, a->seq_q}, 2) ||
+        !row_strides(a->k_stride, {a->batch, a->kv_heads, a->seq_kv}, 2))
         return fail(GAE_ERR_INVALID_ARG, "q and k must be 16-byte aligned, with non-negative strides of 16 bytes");
     for (int i = 0; i < 2; ++i)
         if (a->lse_stride[i] < 0 || a->out_stride[i] < 0)
             return fail(GAE_ERR_INVALID_ARG, "negative lse or out stride");
+    if ((a->batch > 1 && a->out_stride[0] == 0) || (a->kv_heads > 1 && a->out_stride[1] == 0))
+        return fail(GAE_ERR_INVALID_ARG, "output stride of 0");
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (a->seq_q == 0) {
         const int64_t n = a->batch * a->kv_heads * a->seq_kv, blocks = (n + 255) / 256;
@@ -296,10 +310,11 @@ gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
     const bool bf16 = a->dtype == GAE_DTYPE_BF16;
     const int64_t D = a->head_dim;
     const CUtensorMapDataType dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if ((s = make_map_4d(&p.tm_q, a->q, dt, 2, a->batch, a->heads, a->seq_q, D, a->q_stride[0], a->q_stride[1],
-                         a->q_stride[2], 128)) != GAE_OK ||
-        (s = make_map_4d(&p.tm_k, a->k, dt, 2, a->batch, a->kv_heads, a->seq_kv, D, a->k_stride[0], a->k_stride[1],
-                         a->k_stride[2], 128)) != GAE_OK)
+    auto stride = [&](int64_t st, int64_t n) { return n > 1 ? st : D; };  // a map checks the unused ones too
+    if ((s = make_map_4d(&p.tm_q, a->q, dt, 2, a->batch, a->heads, a->seq_q, D, stride(a->q_stride[0], a->batch),
+                         stride(a->q_stride[1], a->heads), stride(a->q_stride[2], a->seq_q), 128)) != GAE_OK ||
+        (s = make_map_4d(&p.tm_k, a->k, dt, 2, a->batch, a->kv_heads, a->seq_kv, D, stride(a->k_stride[0], a->batch),
+                         stride(a->k_stride[1], a->kv_heads), stride(a->k_stride[2], a->seq_kv), 128)) != GAE_OK)
         return s;
     p.lse = a->lse;
     p.l_sb = a->lse_stride[0]; p.l_sh = a->lse_stride[1];
@@ -347,6 +362,8 @@ gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *
     if (!a->seq_lens || !a->new_lens || !a->kept || !a->kept_weights || (a->max_pages > 0 && a->weights_len > 0 && !a->weights))
         return fail(GAE_ERR_INVALID_ARG, "NULL pointer in eviction arguments");
     if (a->page_table == a->dst_table) return fail(GAE_ERR_INVALID_ARG, "dst_table must name other pages than page_table");
+    if (a->new_lens == a->seq_lens || a->kept_weights == a->weights)
+        return fail(GAE_ERR_INVALID_ARG, "eviction cannot write its lengths or weights over those it reads");
     if (a->w_stride[0] < 0 || a->w_stride[1] < 0 || a->weights_len < 0)
         return fail(GAE_ERR_INVALID_ARG, "negative weights stride or length");
     p.lens = a->seq_lens; p.w = a->weights;

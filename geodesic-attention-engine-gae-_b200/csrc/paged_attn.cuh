@@ -46,9 +46,6 @@ struct PagedAttnParams {
     float *part_o;        // [blocks][2][heads of a tile][D]
 };
 
-#ifndef GAE_PA_STAGES
-#define GAE_PA_STAGES 2
-#endif
 constexpr int kPaWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
@@ -372,7 +369,7 @@ struct PaFmaTile {
 template <class Tile, int DM>
 struct PaCfg {
     static constexpr int kSlot = Tile::kKeys * DM * (int)sizeof(typename Tile::Elem) * 2;  // K and V rows of a warp
-    static constexpr int kStages = DM == 64 ? 2 * GAE_PA_STAGES : GAE_PA_STAGES;
+    static constexpr int kStages = DM == 64 ? 4 : 2;
     static constexpr int kRing = kPaWarps * kStages * kSlot;
     static constexpr int kOffMl = kRing;                                   // [warps][heads][2]
     static constexpr int kOffQ = kOffMl + kPaWarps * Tile::kHeads * 8;     // fp32 tiles: q [heads][DM]

@@ -255,9 +255,9 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
         if o is None:
             o = torch.empty_like(q)
         if return_lse and l is None:
-            l = torch.empty((B, H), dtype=torch.float32, device=q.device)
+            l = torch.empty_strided((B, H), (H, 1), dtype=torch.float32, device=q.device)
         n = _attn_workspace(B, H, Hkv, D, cap, weights is not None)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device)
+        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device)  # quicker than empty()
         ob, oh, _ = o.stride()
         a = _pack_attn(q.data_ptr(), o.data_ptr(), 0 if l is None else l.data_ptr(), qb, qh, ob, oh, B, H, *table,
                        lens, 1.0 / math.sqrt(D) if scale is None else scale, w[0], wo[0], *w[1:], *wo[1:], cap,

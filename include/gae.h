@@ -479,9 +479,10 @@ GAE_API gae_status gae_layernorm_fwd(const void *x, const void *res, void *sum_o
  * bf16, f16 or f32, any head_dim <= 256 whose rows are a multiple of 16 bytes,
  * any page_size >= 1, heads a multiple of kv_heads (query head h reads key
  * head h / (heads / kv_heads)).  Pool, row and output pointers are 16-byte
- * aligned and their strides non-negative multiples of 16 bytes.  Two
- * sequences may share pages that are only read.  Every entry point works on
- * the current device, allocates nothing and may be captured into a CUDA graph.
+ * aligned and their strides non-negative multiples of 16 bytes (those of a
+ * dimension of one element are not looked at).  Two sequences may share pages
+ * that are only read.  Every entry point works on the current device, allocates
+ * nothing and may be captured into a CUDA graph.
  * ---------------------------------------------------------------------- */
 typedef struct {
     void *k;
@@ -515,7 +516,9 @@ GAE_API gae_status gae_paged_append(const gae_kv_pool *pool, const gae_paged_app
  * sum_t softmax_t(scale * <q[b, h], k_t>) v_t over t < seq_lens[b] (q, o
  * [batch, heads, head_dim], strides {batch, head}); lse (optional, fp32,
  * contiguous [batch, heads]) as in gae_attn_fwd.  A sequence with no keys has
- * o = 0 and lse = -inf.  Statistics and accumulation in fp32.
+ * o = 0 and lse = -inf.  Statistics and accumulation in fp32; 16-bit
+ * probabilities are held as the sum of two 16-bit numbers (an infinite value
+ * among a sequence's own gives NaN).
  * With weights_out (fp32 [batch, kv_heads, weights_len], strides
  * {batch, head}) the call also adds up the weight of every key:
  * weights_out[b, hk, t] = weights[b, hk, t] + sum over the group's heads of
@@ -590,7 +593,7 @@ GAE_API gae_status gae_key_weights(const gae_key_weights_args *args, void *strea
  * The kept rows are copied in their order to positions 0, 1, ... of dst_table,
  * whose pages must not be among those that the call reads (a free page each;
  * the old pages may be shared and stay as they are).  Outputs, contiguous:
- * new_lens [batch], kept [batch, kv_heads, keep] (positions, -1 beyond the
+ * new_lens [batch] (not seq_lens itself), kept [batch, kv_heads, keep] (positions, -1 beyond the
  * new length) and kept_weights [batch, kv_heads, keep] (0 beyond it).
  * 1 <= keep <= dst_max_pages * page_size, 0 <= recent <= keep. */
 typedef struct {

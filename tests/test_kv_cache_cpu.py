@@ -65,8 +65,8 @@ KEYS = dict(q=PTR, k=PTR, lse=PTR, out=PTR, batch=1, heads=4, kv_heads=2, seq_q=
             q_stride=(4096, 1024, 64), k_stride=(4096, 1024, 64), lse_stride=(64, 16), out_stride=(32, 16), dtype=1,
             scale=0.125, workspace=PTR, workspace_bytes=1 << 30)
 EVICT = dict(batch=1, page_table=PTR, table_stride=4, max_pages=4, seq_lens=PTR, weights=PTR, w_stride=(128, 64),
-             weights_len=64, dst_table=PTR + 4096, dst_stride=2, dst_max_pages=2, keep=32, recent=4, new_lens=PTR,
-             kept=PTR, kept_weights=PTR)
+             weights_len=64, dst_table=PTR + 4096, dst_stride=2, dst_max_pages=2, keep=32, recent=4, new_lens=PTR + 64,
+             kept=PTR, kept_weights=PTR + 64)
 
 POOL_BAD = [(dict(num_pages=-1), INVALID), (dict(kv_heads=0), INVALID), (dict(page_size=0), INVALID),
             (dict(head_dim=0), INVALID), (dict(head_dim=60), UNSUPPORTED), (dict(head_dim=264), UNSUPPORTED),
@@ -95,7 +95,7 @@ def _refused(gae, fn, cls, base, bad, status):
     (dict(batch=-1), INVALID), (dict(tokens=-1), INVALID), (dict(k_new=None), INVALID), (dict(start=None), INVALID),
     (dict(page_table=None), INVALID), (dict(max_pages=-1), INVALID), (dict(table_stride=-4), INVALID),
     (dict(v_new=PTR + 2), INVALID), (dict(k_new_stride=(128, 60, 128)), INVALID),
-    (dict(v_new_stride=(128, 64, -128)), INVALID), (dict(batch=65536), UNSUPPORTED),
+    (dict(v_new_stride=(128, 64, -128), tokens=2), INVALID), (dict(batch=65536), UNSUPPORTED),
     (dict(max_pages=1 << 30), UNSUPPORTED), (dict(tokens=(1 << 30) + 1), UNSUPPORTED)])
 def test_append_refusals(gae, bad, status):
     _refused(gae, "gae_paged_append", gae.PagedAppendArgs, APPEND, bad, status)
@@ -110,6 +110,8 @@ def test_append_refusals(gae, bad, status):
     (dict(weights=PTR, weights_out=PTR, weights_len=64, w_stride=(-1, 0)), INVALID),
     (dict(weights=PTR, weights_out=PTR, weights_len=64, workspace_bytes=16), INVALID),
     (dict(weights=PTR, weights_out=PTR, weights_len=64, workspace=None), INVALID),
+    (dict(o_stride=(256, 0)), INVALID), (dict(batch=2, o_stride=(0, 64)), INVALID),
+    (dict(weights=PTR, weights_out=PTR, weights_len=64, w_out_stride=(64, 0)), INVALID),
     (dict(batch=65536), UNSUPPORTED)])
 def test_attention_refusals(gae, bad, status):
     _refused(gae, "gae_paged_attn_fwd", gae.PagedAttnArgs, ATTN, bad, status)
@@ -119,7 +121,8 @@ def test_attention_refusals(gae, bad, status):
     (dict(batch=0), INVALID), (dict(heads=3), INVALID), (dict(kv_heads=0), INVALID), (dict(seq_q=-1), INVALID),
     (dict(head_dim=96), UNSUPPORTED), (dict(dtype=0), UNSUPPORTED), (dict(q=None), INVALID), (dict(out=None), INVALID),
     (dict(k=PTR + 8), INVALID), (dict(k_stride=(4096, 1024, 60)), INVALID), (dict(lse_stride=(-1, 16)), INVALID),
-    (dict(scale=-0.5), UNSUPPORTED), (dict(batch=20000), UNSUPPORTED)])
+    (dict(scale=-0.5), UNSUPPORTED), (dict(batch=20000), UNSUPPORTED),
+    (dict(out_stride=(32, 0)), INVALID), (dict(workspace_bytes=0, workspace=None, seq_q=1 << 16), INVALID)])
 def test_key_weights_refusals(gae, bad, status):
     a = _args(gae.KeyWeightsArgs, KEYS, **bad)
     assert gae.lib().gae_key_weights(C.byref(a), None) == status
@@ -129,7 +132,8 @@ def test_key_weights_refusals(gae, bad, status):
     (dict(batch=-1), INVALID), (dict(keep=0), INVALID), (dict(recent=-1), INVALID), (dict(recent=33), INVALID),
     (dict(keep=33), INVALID), (dict(dst_table=PTR), INVALID), (dict(weights=None), INVALID), (dict(kept=None), INVALID),
     (dict(seq_lens=None), INVALID), (dict(w_stride=(-1, 0)), INVALID), (dict(weights_len=-1), INVALID),
-    (dict(dst_table=None), INVALID), (dict(batch=65536), UNSUPPORTED)])
+    (dict(dst_table=None), INVALID), (dict(batch=65536), UNSUPPORTED), (dict(new_lens=PTR, seq_lens=PTR), INVALID),
+    (dict(kept_weights=PTR, weights=PTR), INVALID)])
 def test_evict_refusals(gae, bad, status):
     _refused(gae, "gae_paged_evict", gae.PagedEvictArgs, EVICT, bad, status)
 

@@ -224,6 +224,40 @@ def test_attention_is_the_same_every_time(gae):
         assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
 
 
+def test_attention_of_nothing(gae):
+    """No sequences, no pages to a sequence, no pages at all."""
+    g, D = _gen(10), 64
+    k, v = _pools(4, 2, 16, D, torch.bfloat16, g)
+    z = lambda *s: torch.zeros(*s, dtype=torch.int32, device="cuda")  # noqa: E731
+    q = torch.randn(3, 4, D, device="cuda", generator=g).bfloat16()
+    assert gae.paged_attention(q[:0], k, v, z(0, 5), z(0)).shape == (0, 4, D)
+    for kk, table in ((k, z(3, 0)), (k[:0], z(3, 5))):
+        w = torch.rand(3, 2, 80, device="cuda")
+        was = w.clone()
+        out, lse = gae.paged_attention(q, kk, kk, table, z(3) + 50, return_lse=True, weights=w)
+        assert (out == 0).all() and (lse == -math.inf).all() and torch.equal(w, was)
+    gae.paged_append(q[:, :2, None], q[:, :2, None], k[:0], v[:0], z(3, 5), z(3))
+    new, kept, kw = gae.paged_evict(k[:0], v[:0], z(3, 5), z(3) + 9, torch.rand(3, 2, 80, device="cuda"), z(3, 1), keep=4)
+    assert (new == 0).all() and (kept == -1).all() and (kw == 0).all()
+
+
+def test_strides_of_single_elements_are_not_looked_at(gae):
+    g, D = _gen(11), 64
+    odd = lambda t, *st: t.as_strided(t.shape, st)  # noqa: E731
+    k, v = _pools(1, 1, 32, D, torch.bfloat16, g)
+    k, v = odd(k, 7, 3, D, 1), odd(v, 5, 1, D, 1)
+    q = odd(torch.randn(1, 1, D, device="cuda", generator=g).bfloat16(), 3, 9, 1)
+    table, lens = torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.tensor([20], dtype=torch.int32, device="cuda")
+    _check_attention(gae, q, k, v, table, lens)
+    new = odd(torch.randn(1, 1, 1, D, device="cuda", generator=g).bfloat16(), 1, 3, 5, 1)
+    gae.paged_append(new, new, k, v, table, lens)
+    assert torch.equal(k[0, 0, 20], new[0, 0, 0])
+    qk, kk = odd(q[:, :, None].clone(), 3, 5, 7, 1), odd(k[:, :, :20].clone(), 1, 3, D, 1)
+    lse = torch.zeros(1, 1, 1, device="cuda")
+    w = gae.attention_key_weights(qk, kk, lse)
+    _check_keys(gae, qk, kk, lse, w, False, 0)
+
+
 # ------------------------------------------------------------------ append
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("D,Hkv,page,T,layout", [(64, 12, 16, 1, "heads"), (128, 2, 7, 45, "slots"), (8, 1, 1, 9, "heads"),
