@@ -583,8 +583,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
         tile.load_q(row.q, p.q_sh, row.heads, p.pool.D, lane);
     };
     auto stage_q = [&] {  // the fp32 tiles' q
-        if (!Cfg::kQ) return;
-        for (int i = tid; i < Tile::kHeads * DM; i += kThreads) {
+        for (int i = tid; i < (Cfg::kQ ? Tile::kHeads * DM : 0); i += kThreads) {
             const int h = i / DM, d = i % DM;
             q_smem[i] = (h < row.heads && d < p.pool.D) ? to_f<T>(row.q[h * p.q_sh + d]) : 0.f;
         }

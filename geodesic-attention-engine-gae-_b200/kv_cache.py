@@ -26,6 +26,9 @@ from . import GAEError, _check, _torch, lib
 
 _I64_2, _I64_3 = C.c_int64 * 2, C.c_int64 * 3
 
+# Small calls take as long as their host side: argument blocks are packed in one
+# call, and tensors made by empty_strided, the quickest of torch's constructors.
+
 
 class KvPool(C.Structure):
     """Mirror of gae_kv_pool (include/gae.h)."""
@@ -96,26 +99,28 @@ def _bind(L):
     L.gae_key_weights.argtypes = [vp, vp]
 
 
+# The workspaces' sizes, by the calls' sizes alone.
 @functools.lru_cache(maxsize=1024)
 def _attn_workspace(*sizes):
     return lib().gae_paged_attn_workspace_bytes(*sizes)
 
 
-def _run(what, tensors, stream, body):
+@functools.lru_cache(maxsize=1024)
+def _keys_workspace(*sizes):
+    return lib().gae_key_weights_workspace_bytes(*sizes)
+
+
+def _run(what, names, tensors, stream, body):
     """body(stream pointer) with the tensors' device and `stream` current, so that
     what it allocates belongs to the stream it runs on; on a stream other than
-    the current one the inputs are marked as used there.  tensors: by name, the
-    first one's device is everyone's."""
+    the current one the inputs are marked as used there.  The first tensor's
+    device is everyone's; names is for the error that says whose is not."""
     torch = _torch()
-    dev = -2
-    for name, t in tensors:
-        if t is not None:
-            i = t.get_device()
-            if dev == -2:
-                dev = i
-            if i != dev or i < 0:
-                raise GAEError(1, f"{what}: tensors must be on one CUDA device, {name} is on {t.device}")
-    if stream is None and torch.cuda.current_device() == dev:
+    dev = tensors[0].get_device()
+    for i, t in enumerate(tensors):
+        if t is not None and t.get_device() != dev or dev < 0:
+            raise GAEError(1, f"{what}: tensors must be on one CUDA device, {names.split()[i]} is on {t.device}")
+    if stream is None and torch._C._cuda_getDevice() == dev:
         return body(torch._C._cuda_getCurrentRawStream(dev))
     with torch.cuda.device(dev):
         if stream is None:
@@ -123,7 +128,7 @@ def _run(what, tensors, stream, body):
         if stream.device.index != dev:
             raise GAEError(1, f"{what}: stream on {stream.device}, tensors on device {dev}")
         with torch.cuda.stream(stream):
-            for _, t in tensors:
+            for t in tensors:
                 if t is not None:
                     t.record_stream(stream)
             return body(stream.cuda_stream)
@@ -206,8 +211,8 @@ def paged_append(k_new, v_new, k_pages, v_pages, page_table, start, *, counts=No
     a = _pack_append(k_new.data_ptr(), v_new.data_ptr(), kb, kh, kt, vb, vh, vt, B, T,
                      *_table(what, page_table, B), _ints(what, start, B, "start"),
                      0 if counts is None else _ints(what, counts, B, "counts"))
-    _run(what, (("k_pages", k_pages), ("v_pages", v_pages), ("k_new", k_new), ("v_new", v_new),
-                ("page_table", page_table), ("start", start), ("counts", counts)), stream,
+    _run(what, "k_pages v_pages k_new v_new page_table start counts",
+         (k_pages, v_pages, k_new, v_new, page_table, start, counts), stream,
          lambda st: _check(lib().gae_paged_append(pool, a, st)))
 
 
@@ -257,7 +262,7 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
         if return_lse and l is None:
             l = torch.empty_strided((B, H), (H, 1), dtype=torch.float32, device=q.device)
         n = _attn_workspace(B, H, Hkv, D, cap, weights is not None)
-        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device)  # quicker than empty()
+        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device)
         ob, oh, _ = o.stride()
         a = _pack_attn(q.data_ptr(), o.data_ptr(), 0 if l is None else l.data_ptr(), qb, qh, ob, oh, B, H, *table,
                        lens, 1.0 / math.sqrt(D) if scale is None else scale, w[0], wo[0], *w[1:], *wo[1:], cap,
@@ -265,9 +270,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
         _check(L.gae_paged_attn_fwd(pool, a, st))
         return (o, l) if return_lse else o
 
-    return _run(what, (("q", q), ("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
-                       ("seq_lens", seq_lens), ("out", out), ("lse", lse), ("weights", weights),
-                       ("weights_out", weights_out)), stream, body)
+    return _run(what, "q k_pages v_pages page_table seq_lens out lse weights weights_out",
+                (q, k_pages, v_pages, page_table, seq_lens, out, lse, weights, weights_out), stream, body)
 
 
 def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv_offset=0, out=None,
@@ -302,9 +306,11 @@ def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv
     L = lib()
 
     def body(st):
-        w = torch.empty((B, Hkv, Nkv), dtype=torch.float32, device=q.device) if out is None else out
-        n = L.gae_key_weights_workspace_bytes(B, H, Hkv, Nq, Nkv)
-        ws = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
+        w = out
+        if w is None:
+            w = torch.empty_strided((B, Hkv, Nkv), (Hkv * Nkv, Nkv, 1), dtype=torch.float32, device=q.device)
+        n = _keys_workspace(B, H, Hkv, Nq, Nkv)
+        ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device) if n else None
         wp, wb, wh = _weights(what, w, B, Hkv, Nkv, "out")
         a = _pack_keys(q.data_ptr(), k.data_ptr(), l[0], wp, B, H, Hkv, Nq, Nkv, D, qb, qh, qn, kb, kh, kn,
                        *l[1:], wb, wh, _code(q), 1 if causal else 0, 1 if accumulate else 0,
@@ -313,7 +319,7 @@ def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv
         _check(L.gae_key_weights(a, st))
         return w
 
-    return _run(what, (("q", q), ("k", k), ("lse", lse), ("out", out)), stream, body)
+    return _run(what, "q k lse out", (q, k, lse, out), stream, body)
 
 
 def paged_evict(k_pages, v_pages, page_table, seq_lens, weights, dst_table, *, keep, recent=0, stream=None):
@@ -338,15 +344,16 @@ def paged_evict(k_pages, v_pages, page_table, seq_lens, weights, dst_table, *, k
     def body(st):
         dev = k_pages.device
         new_lens = torch.empty_like(seq_lens)
-        kept = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
-        kept_w = torch.empty((B, Hkv, keep), dtype=torch.float32, device=dev)
+        shape, strides = (B, Hkv, keep), (Hkv * keep, keep, 1)
+        kept = torch.empty_strided(shape, strides, dtype=torch.int32, device=dev)
+        kept_w = torch.empty_strided(shape, strides, dtype=torch.float32, device=dev)
         a = _pack_evict(B, *table, lens, *w, weights.shape[2], *dst, keep, recent, new_lens.data_ptr(),
                         kept.data_ptr(), kept_w.data_ptr())
         _check(lib().gae_paged_evict(pool, a, st))
         return new_lens, kept, kept_w
 
-    return _run(what, (("k_pages", k_pages), ("v_pages", v_pages), ("page_table", page_table),
-                       ("seq_lens", seq_lens), ("weights", weights), ("dst_table", dst_table)), stream, body)
+    return _run(what, "k_pages v_pages page_table seq_lens weights dst_table",
+                (k_pages, v_pages, page_table, seq_lens, weights, dst_table), stream, body)
 
 
 class PagedKVCache:
