@@ -123,7 +123,7 @@ struct EvictParams {
     int *new_lens;        // [B]
     int *kept;            // [B, Hkv, keep]
     float *w_out;         // [B, Hkv, keep]
-    int chunks;
+    int chunks, esize;    // 16-byte pieces of a row, bytes of an element
 };
 
 // Whole-number order of the weights: NaN above +inf, -0 equal to 0.  Every
@@ -135,13 +135,69 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return (u >> 31) ? ~u : (u | 0x80000000u);
 }
 
+// Kept rows first, first + step, ... of (b, hk), their 16-byte piece c of K and
+// V, to the same positions of the destination table: kRows copies on their
+// way at once.
+constexpr int kGatherRows = 4;
+
+template <int kRows>
+__device__ __forceinline__ void evict_gather(const EvictParams &p, int b, int hk, int first, int step, int c) {
+    const int *kept = p.kept + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
+    char *k = static_cast<char *>(p.pool.k) + hk * p.pool.k_sh * p.esize + c * 16;
+    char *v = static_cast<char *>(p.pool.v) + hk * p.pool.v_sh * p.esize + c * 16;
+    int from[kRows], page[kRows], to_page[kRows];
+    int4 x[kRows], y[kRows];
+#pragma unroll
+    for (int e = 0; e < kRows; ++e) from[e] = first + e * step < p.keep ? kept[first + e * step] : -1;
+#pragma unroll
+    for (int e = 0; e < kRows; ++e) {
+        page[e] = to_page[e] = -1;
+        if (from[e] < 0) continue;
+        const uint32_t idx = p.pool.by_page.div(from[e]);
+        page[e] = page_of(p.src, p.pool.num_pages, b, (int)idx);
+        from[e] -= (int)idx * p.pool.page;
+        to_page[e] = page_of(p.dst, p.pool.num_pages, b, (int)p.pool.by_page.div((uint32_t)(first + e * step)));
+    }
+#pragma unroll
+    for (int e = 0; e < kRows; ++e)
+        if (page[e] >= 0) {
+            x[e] = *reinterpret_cast<const int4 *>(k + (page[e] * p.pool.k_sp + from[e] * p.pool.k_ss) * p.esize);
+            y[e] = *reinterpret_cast<const int4 *>(v + (page[e] * p.pool.v_sp + from[e] * p.pool.v_ss) * p.esize);
+        }
+#pragma unroll
+    for (int e = 0; e < kRows; ++e)
+        if (page[e] >= 0 && to_page[e] >= 0) {
+            const uint32_t to = (uint32_t)(first + e * step);
+            const int64_t slot = to - (int64_t)p.pool.by_page.div(to) * p.pool.page;
+            *reinterpret_cast<int4 *>(k + (to_page[e] * p.pool.k_sp + slot * p.pool.k_ss) * p.esize) = x[e];
+            *reinterpret_cast<int4 *>(v + (to_page[e] * p.pool.v_sp + slot * p.pool.v_ss) * p.esize) = y[e];
+        }
+}
+
+// The weights of kept positions first, first + step, ...; 0 beyond the length.
+template <int kRows>
+__device__ __forceinline__ void evict_weights(const EvictParams &p, int b, int hk, int first, int step) {
+    const int64_t row = ((int64_t)b * p.pool.Hkv + hk) * p.keep;
+    const float *w = p.w + b * p.w_sb + hk * p.w_sh;
+#pragma unroll
+    for (int e = 0; e < kRows; ++e) {
+        const int i = first + e * step;
+        if (i >= p.keep) break;
+        const int pos = p.kept[row + i];
+        p.w_out[row + i] = pos >= 0 ? __ldg(w + pos) : 0.f;
+    }
+}
+
 // The keep-th largest key of a (key head, sequence) row is found by a radix
 // search over its 11, 11 and 10 highest bits; positions above it, and the first
 // of those equal to it, are then listed in ascending order.  A cluster of up to
 // 8 CTAs shares a row where there are few rows, each with its run of positions: the keys are formed once
 // and stay in shared memory (positions beyond kMaxKeys are formed again), only
 // histograms and counts cross the cluster.  What bounds it is latency: one
-// barrier of the cluster to a digit.
+// barrier of the cluster to a digit.  Where a row's CTAs have little to copy
+// they do it themselves (a launch less: 18 -> 16.4 us at 1024 positions of two
+// sequences x 12 heads); larger shares are left to a kernel that fills the GPU
+// (50000 positions to 8192: 71 us either way, of which the copies take 43).
 constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32, kEvictBins = 2048;
 constexpr int kEvictMaxCluster = 8, kEvictMaxKeys = 40960;
 
@@ -160,7 +216,7 @@ __device__ __forceinline__ uint2 ld_cluster_u2(uint32_t addr, uint32_t rank) {
     return v;
 }
 
-__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictParams p, int cluster, int max_keys) {
+__global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const EvictParams p, int cluster, int max_keys, int copy) {
     extern __shared__ __align__(16) uint32_t smem_ev[];
     uint32_t *hist = smem_ev;                    // [2][bins], one digit's after the other's
     uint32_t *keys = smem_ev + 2 * kEvictBins;  // [max_keys], a multiple of 4
@@ -338,65 +394,32 @@ __global__ void __launch_bounds__(kEvictThreads) evict_select_kernel(const Evict
         }
     for (int i = n_keep + rank * kEvictThreads + tid; i < p.keep; i += cluster * kEvictThreads) kept[i] = -1;
     if (hk == 0 && rank == 0 && tid == 0) p.new_lens[b] = n_keep;
-    // no CTA leaves while another reads its counts
-    asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
-}
-
-// Kept row i of (b, hk) -> position i of the destination table's pages, K and V,
-// and its weight beside its position; 16 bytes to a thread and row, kGatherRows rows at once: that many copies on
-// their way are what the memory needs.
-constexpr int kGatherRows = 4;
-
-template <int ESIZE>
-__global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int hk = blockIdx.y, b = blockIdx.z, rows = 256 / p.chunks;  // rows of a pass of the block
-    const int c = threadIdx.x % p.chunks, r = threadIdx.x / p.chunks;
-    const int *kept = p.kept + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
-    const int weight_blocks = (p.keep + 1023) / 1024;
-    if ((int)blockIdx.x < weight_blocks) {  // the first blocks: 1024 weights each
-        const float *w = p.w + b * p.w_sb + hk * p.w_sh;
-        float *wo = p.w_out + ((int64_t)b * p.pool.Hkv + hk) * p.keep;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int i = blockIdx.x * 1024 + e * 256 + threadIdx.x;
-            if (i >= p.keep) break;
-            const int pos = kept[i];
-            wo[i] = pos >= 0 ? __ldg(w + pos) : 0.f;
-        }
+    if (!copy) {
+        // no CTA leaves while another reads its counts
+        asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
         return;
     }
-    if (r >= rows) return;
-    const int64_t first = (int64_t)(blockIdx.x - weight_blocks) * rows * kGatherRows + r;
-    const char *k = static_cast<const char *>(p.pool.k) + hk * p.pool.k_sh * ESIZE + c * 16;
-    const char *v = static_cast<const char *>(p.pool.v) + hk * p.pool.v_sh * ESIZE + c * 16;
-    int from[kGatherRows], page[kGatherRows], to_page[kGatherRows];
-    int4 x[kGatherRows], y[kGatherRows];
-#pragma unroll
-    for (int e = 0; e < kGatherRows; ++e) from[e] = first + e * rows < p.keep ? kept[first + e * rows] : -1;
-#pragma unroll
-    for (int e = 0; e < kGatherRows; ++e) {
-        page[e] = to_page[e] = -1;
-        if (from[e] < 0) continue;
-        const uint32_t idx = p.pool.by_page.div(from[e]);
-        page[e] = page_of(p.src, p.pool.num_pages, b, (int)idx);
-        from[e] -= (int)idx * p.pool.page;
-        to_page[e] = page_of(p.dst, p.pool.num_pages, b, (int)p.pool.by_page.div((uint32_t)(first + e * rows)));
+    cluster_publish();  // the row's list is complete
+    for (int i = rank * kEvictThreads + tid; i < p.keep; i += cluster * kEvictThreads) evict_weights<1>(p, b, hk, i, 0);
+    const int rows = kEvictThreads / p.chunks, r = tid / p.chunks;
+    if (r < rows)
+        for (int i = rank * rows * 2 + r; i < n_keep; i += cluster * rows * 2)
+            evict_gather<2>(p, b, hk, i, rows, tid % p.chunks);
+}
+
+// The copies of a large share: blocks of their own, the first ones the weights,
+// 1024 each.
+__global__ void __launch_bounds__(256) evict_gather_kernel(const EvictParams p) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int hk = blockIdx.y, b = blockIdx.z, weight_blocks = (p.keep + 1023) / 1024;
+    if ((int)blockIdx.x < weight_blocks) {
+        evict_weights<4>(p, b, hk, blockIdx.x * 1024 + threadIdx.x, 256);
+        return;
     }
-#pragma unroll
-    for (int e = 0; e < kGatherRows; ++e)
-        if (page[e] >= 0) {
-            x[e] = *reinterpret_cast<const int4 *>(k + (page[e] * p.pool.k_sp + from[e] * p.pool.k_ss) * ESIZE);
-            y[e] = *reinterpret_cast<const int4 *>(v + (page[e] * p.pool.v_sp + from[e] * p.pool.v_ss) * ESIZE);
-        }
-#pragma unroll
-    for (int e = 0; e < kGatherRows; ++e)
-        if (page[e] >= 0 && to_page[e] >= 0) {
-            const int64_t to = first + e * rows;
-            const int64_t slot = to - (int64_t)p.pool.by_page.div((uint32_t)to) * p.pool.page;
-            *reinterpret_cast<int4 *>(const_cast<char *>(k) + (to_page[e] * p.pool.k_sp + slot * p.pool.k_ss) * ESIZE) = x[e];
-            *reinterpret_cast<int4 *>(const_cast<char *>(v) + (to_page[e] * p.pool.v_sp + slot * p.pool.v_ss) * ESIZE) = y[e];
-        }
+    const int rows = 256 / p.chunks, r = threadIdx.x / p.chunks;
+    if (r < rows)
+        evict_gather<kGatherRows>(p, b, hk, (int)(blockIdx.x - weight_blocks) * rows * kGatherRows + r, rows,
+                                  threadIdx.x % p.chunks);
 }
 
 }  // namespace gae

@@ -372,6 +372,7 @@ gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *
     p.new_lens = a->new_lens; p.kept = a->kept; p.w_out = a->kept_weights;
     const int es = dtype_size(pool->dtype);
     p.chunks = (int)(pool->head_dim * es / 16);
+    p.esize = es;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     // As many CTAs to a row as the GPU has room for beside the other rows', each
     // with 4096 positions at least; more where a CTA could not hold its keys.
@@ -398,11 +399,15 @@ gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *
     at.val.clusterDim.y = at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    GAE_CUDA_TRY(cudaLaunchKernelEx(&cfg, gae::evict_select_kernel, (const gae::EvictParams)p, cluster, max_keys));
+    // A row's own CTAs copy what it keeps where that is little to each; else
+    // blocks of their own do.
+    const int copy = a->keep * pool->head_dim * es * 2 / cluster <= (256 << 10);
+    GAE_CUDA_TRY(cudaLaunchKernelEx(&cfg, gae::evict_select_kernel, (const gae::EvictParams)p, cluster, max_keys, copy));
+    if (copy) return GAE_OK;
     const int64_t block_rows = 256 / p.chunks * gae::kGatherRows;
-    const dim3 grid((unsigned)((a->keep + block_rows - 1) / block_rows + (a->keep + 1023) / 1024), (unsigned)pool->kv_heads, (unsigned)a->batch);
-    return es == 4 ? launch_after(gae::evict_gather_kernel<4>, grid, 256, st, p)
-                   : launch_after(gae::evict_gather_kernel<2>, grid, 256, st, p);
+    const dim3 grid((unsigned)((a->keep + block_rows - 1) / block_rows + (a->keep + 1023) / 1024), (unsigned)pool->kv_heads,
+                    (unsigned)a->batch);
+    return launch_after(gae::evict_gather_kernel, grid, 256, st, p);
 }
 
 }  // extern "C"
