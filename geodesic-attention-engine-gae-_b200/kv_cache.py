@@ -99,6 +99,13 @@ def _bind(L):
     L.gae_key_weights.argtypes = [vp, vp]
 
 
+@functools.lru_cache(maxsize=None)
+def _load():
+    """torch, imported by the first call; the dtypes' codes; int32; float32."""
+    torch = _torch()
+    return torch, {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}, torch.int32, torch.float32
+
+
 # The workspaces' sizes, by the calls' sizes alone.
 @functools.lru_cache(maxsize=1024)
 def _attn_workspace(*sizes):
@@ -115,11 +122,12 @@ def _run(what, names, tensors, stream, body):
     what it allocates belongs to the stream it runs on; on a stream other than
     the current one the inputs are marked as used there.  The first tensor's
     device is everyone's; names is for the error that says whose is not."""
-    torch = _torch()
+    torch = _load()[0]
     dev = tensors[0].get_device()
-    for i, t in enumerate(tensors):
+    for t in tensors:
         if t is not None and t.get_device() != dev or dev < 0:
-            raise GAEError(1, f"{what}: tensors must be on one CUDA device, {names.split()[i]} is on {t.device}")
+            name = names.split()[next(i for i, x in enumerate(tensors) if x is t)]
+            raise GAEError(1, f"{what}: tensors must be on one CUDA device, {name} is on {t.device}")
     if stream is None and torch._C._cuda_getDevice() == dev:
         return body(torch._C._cuda_getCurrentRawStream(dev))
     with torch.cuda.device(dev):
@@ -134,15 +142,8 @@ def _run(what, names, tensors, stream, body):
             return body(stream.cuda_stream)
 
 
-_CODES = None
-
-
 def _code(t):
-    global _CODES
-    if _CODES is None:
-        torch = _torch()
-        _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-    c = _CODES.get(t.dtype)
+    c = _load()[1].get(t.dtype)
     if c is None:
         raise GAEError(1, f"unsupported dtype {t.dtype}")
     return c
@@ -164,7 +165,7 @@ def _pool(what, k_pages, v_pages):
 
 def _table(what, table, batch, name="page_table"):
     shape = table.shape
-    if len(shape) != 2 or shape[0] != batch or table.dtype != _torch().int32:
+    if len(shape) != 2 or shape[0] != batch or table.dtype != _load()[2]:
         raise GAEError(1, f"{what}: {name} must be int32 [batch, max_pages]")
     row, one = table.stride()
     if one != 1 and shape[1] > 1:
@@ -173,7 +174,7 @@ def _table(what, table, batch, name="page_table"):
 
 
 def _ints(what, t, batch, name):
-    if t.dtype != _torch().int32 or t.shape != (batch,) or not t.is_contiguous():
+    if t.dtype != _load()[2] or t.shape != (batch,) or not t.is_contiguous():
         raise GAEError(1, f"{what}: {name} must be contiguous int32 [batch]")
     return t.data_ptr()
 
@@ -181,7 +182,7 @@ def _ints(what, t, batch, name):
 def _weights(what, t, batch, heads, n, name):
     """(address, batch stride, head stride)"""
     shape = t.shape
-    if len(shape) != 3 or shape[0] != batch or shape[1] != heads or shape[2] < n or t.dtype != _torch().float32:
+    if len(shape) != 3 or shape[0] != batch or shape[1] != heads or shape[2] < n or t.dtype != _load()[3]:
         raise GAEError(1, f"{what}: {name} must be fp32 [{batch}, {heads}, >= {n}]")
     sb, sh, one = t.stride()
     if one != 1 and shape[2] > 1:
@@ -228,7 +229,7 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
     head's query heads; weights_out defaults to weights (in place).  Positions
     without a key are left as they are."""
     what = "paged_attention"
-    torch = _torch()
+    torch = _load()[0]
     shape = q.shape
     if len(shape) != 3:
         raise GAEError(1, f"{what}: q must be [batch, heads, head_dim]")
@@ -265,7 +266,7 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
         ws = torch.empty_strided((n,), (1,), dtype=torch.uint8, device=q.device)
         ob, oh, _ = o.stride()
         a = _pack_attn(q.data_ptr(), o.data_ptr(), 0 if l is None else l.data_ptr(), qb, qh, ob, oh, B, H, *table,
-                       lens, 1.0 / math.sqrt(D) if scale is None else scale, w[0], wo[0], *w[1:], *wo[1:], cap,
+                       lens, 1.0 / math.sqrt(D) if scale is None else float(scale), w[0], wo[0], *w[1:], *wo[1:], cap,
                        ws.data_ptr(), n)
         _check(L.gae_paged_attn_fwd(pool, a, st))
         return (o, l) if return_lse else o
@@ -284,7 +285,7 @@ def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv
     queries is q[:, :, -n:], lse[:, :, -n:] with q_offset = N - n.  out may be a
     view of a cache's weights; accumulate=True adds to it."""
     what = "attention_key_weights"
-    torch = _torch()
+    torch = _load()[0]
     qs, ks = q.shape, k.shape
     if len(qs) != 4 or len(ks) != 4:
         raise GAEError(1, f"{what}: q and k must be [batch, heads, seq, head_dim]")
@@ -314,7 +315,7 @@ def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv
         wp, wb, wh = _weights(what, w, B, Hkv, Nkv, "out")
         a = _pack_keys(q.data_ptr(), k.data_ptr(), l[0], wp, B, H, Hkv, Nq, Nkv, D, qb, qh, qn, kb, kh, kn,
                        *l[1:], wb, wh, _code(q), 1 if causal else 0, 1 if accumulate else 0,
-                       1.0 / math.sqrt(D) if scale is None else scale, q_offset, kv_offset,
+                       1.0 / math.sqrt(D) if scale is None else float(scale), q_offset, kv_offset,
                        ws.data_ptr() if n else 0, n)
         _check(L.gae_key_weights(a, st))
         return w
@@ -331,7 +332,7 @@ def paged_evict(k_pages, v_pages, page_table, seq_lens, weights, dst_table, *, k
     positions int32 [B, Hkv, keep], -1 beyond the length, their weights fp32,
     0 beyond)."""
     what = "paged_evict"
-    torch = _torch()
+    torch = _load()[0]
     pool, (_, Hkv, _, _) = _pool(what, k_pages, v_pages)
     B = page_table.shape[0]
     table = _table(what, page_table, B)

@@ -479,6 +479,29 @@ def test_on_another_stream_and_captured(gae):
     _check_attention(gae, q, k, v, table, lens, got=r1)
     _check_attention(gae, q.flip(0), k, v, table, lens, got=r2)
 
+    # append, key weights and eviction on a stream of their own, the weights a slice of a wider buffer
+    rows = torch.randn(B, Hkv, 5, D, device="cuda", generator=g).bfloat16()
+    wide = torch.rand(B, Hkv, M * page + 3, device="cuda", generator=g)
+    part = wide[:, :, 3:]
+    lse = torch.full((B, 8, 70), 6.0, device="cuda")
+    qq, kk = (torch.randn(B, h, n, D, device="cuda", generator=g).bfloat16() for h, n in ((8, 70), (Hkv, 90)))
+    torch.cuda.synchronize()
+    gae.paged_append(rows, -rows, k, v, table, lens, stream=s1)
+    was = part.clone()
+    s1.synchronize()
+    o2 = gae.paged_attention(q, k, v, table, lens + 5, return_lse=True, weights=part, stream=s1)
+    kw2 = gae.attention_key_weights(qq, kk, lse, causal=True, q_offset=20, stream=s1)
+    s1.synchronize()
+    ref = _evict_reference(k.cpu(), v.cpu(), table.cpu(), lens.cpu(), part.cpu(), dst.cpu(), 90, 3)
+    e2 = gae.paged_evict(k, v, table, lens, part, dst, keep=90, recent=3, stream=s1)
+    torch.cuda.synchronize()
+    for b, n in enumerate(lens.tolist()):
+        assert torch.equal(k[table[b, (n + 4) // page].long(), :, (n + 4) % page], rows[b, :, 4])
+    _check_attention(gae, q, k, v, table, lens + 5, got=o2)
+    assert ((part - was).sum(-1) - 4).abs().max() <= 1e-3  # four query heads' weights of one each
+    _check_keys(gae, qq, kk, lse, kw2, True, 20)
+    assert torch.equal(e2[1].cpu(), ref[3]) and torch.equal(k.cpu(), ref[0]) and torch.equal(v.cpu(), ref[1])
+
     new = torch.randn(B, Hkv, 1, D, device="cuda", generator=g).bfloat16()
     after = lens + 1
     w2 = w.clone()
