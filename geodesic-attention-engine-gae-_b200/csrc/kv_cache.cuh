@@ -195,8 +195,8 @@ __device__ __forceinline__ void evict_weights(const EvictParams &p, int b, int h
 // and stay in shared memory (positions beyond kMaxKeys are formed again), only
 // histograms and counts cross the cluster.  What bounds it is latency: one
 // barrier of the cluster to a digit.  Where a row's CTAs have little to copy
-// they do it themselves (a launch less: 18 -> 16.4 us at 1024 positions of two
-// sequences x 12 heads); larger shares are left to a kernel that fills the GPU
+// they do it themselves (a launch less: 18 -> 16.4 us a call at 1024 positions of
+// two sequences x 12 heads, though 13 -> 15 us replayed from a graph); larger shares are left to a kernel that fills the GPU
 // (50000 positions to 8192: 71 us either way, of which the copies take 43).
 constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32, kEvictBins = 2048;
 constexpr int kEvictMaxCluster = 8, kEvictMaxKeys = 40960;
