@@ -191,13 +191,14 @@ __device__ __forceinline__ void evict_weights(const EvictParams &p, int b, int h
 // The keep-th largest key of a (key head, sequence) row is found by a radix
 // search over its 11, 11 and 10 highest bits; positions above it, and the first
 // of those equal to it, are then listed in ascending order.  A cluster of up to
-// 8 CTAs shares a row where there are few rows, each with its run of positions: the keys are formed once
-// and stay in shared memory (positions beyond kMaxKeys are formed again), only
-// histograms and counts cross the cluster.  What bounds it is latency: one
-// barrier of the cluster to a digit.  Where a row's CTAs have little to copy
-// they do it themselves (a launch less: 18 -> 16.4 us a call at 1024 positions of
-// two sequences x 12 heads, though 13 -> 15 us replayed from a graph); larger shares are left to a kernel that fills the GPU
-// (50000 positions to 8192: 71 us either way, of which the copies take 43).
+// 8 CTAs shares a row where there are few rows, each with its run of positions:
+// the keys are formed once and stay in shared memory (positions beyond
+// kEvictMaxKeys are formed again), only histograms and counts cross the cluster.
+// What bounds it is latency: one barrier of the cluster to a digit.
+// Where a row's CTAs have little to copy they do it themselves (a launch less:
+// 18 -> 16.4 us a call at 1024 positions of two sequences x 12 heads, though 13
+// -> 15 us replayed from a graph); larger shares are left to a kernel that fills
+// the GPU (50000 positions to 8192: 69 us, of which the copies take 43).
 constexpr int kEvictThreads = 1024, kEvictWarps = kEvictThreads / 32, kEvictBins = 2048;
 constexpr int kEvictMaxCluster = 8, kEvictMaxKeys = 40960;
 

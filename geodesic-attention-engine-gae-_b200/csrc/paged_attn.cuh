@@ -47,6 +47,7 @@ struct PagedAttnParams {
     int64_t wi_sb, wi_sh, wo_sb, wo_sh;
     int B, H, G, cap;     // G = H / Hkv, cap = max_pages * page_size
     int groups;           // rows of a key head: ceil(G / heads of a tile)
+    int whole_rows;       // a block to a row, no join
     float scale_log2;
     // workspace
     int2 *parts;          // [rows] first and last block of the row
@@ -411,50 +412,64 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
     auto tiles_of = [&](int len) { return max(1, (len + kTileKeys - 1) / kTileKeys); };  // an empty row is a tile too
 
     // --- this block's run of tiles: [begin, end) of the total
-    int64_t *scan = reinterpret_cast<int64_t *>(smem_pa + Cfg::kOffScan);  // [4] warp sums
-    int *found = reinterpret_cast<int *>(scan + 4);                        // b, r, tile
-    const int per = (p.B + kThreads - 1) / kThreads;
-    const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
-    int64_t mine = 0;
-    for (int b = b0; b < b1; ++b) mine += tiles_of(clamp_len(__ldg(p.lens + b), p.cap));
-    mine *= R;
-    int64_t incl = mine;
-#pragma unroll
-    for (int s = 1; s < 32; s <<= 1) {
-        const int64_t up = __shfl_up_sync(0xffffffffu, incl, s);
-        if (lane >= s) incl += up;
-    }
-    if (lane == 31) scan[warp] = incl;
-    __syncthreads();
-    int64_t excl = incl - mine, total = 0;
-#pragma unroll
-    for (int w = 0; w < kPaWarps; ++w) {
-        if (w < warp) excl += scan[w];
-        total += scan[w];
-    }
-    const int64_t blocks = min64(gridDim.x, total);  // none of them without a tile
-    if (blockIdx.x >= blocks) return;
-    const int64_t begin = total * blockIdx.x / blocks, end = total * (blockIdx.x + 1) / blocks;
-    if (begin >= excl && begin < excl + mine) {
-        int64_t at = excl;
-        for (int b = b0; b < b1; ++b) {
-            const int t = tiles_of(clamp_len(__ldg(p.lens + b), p.cap));
-            if (begin < at + (int64_t)t * R) {
-                found[0] = b;
-                found[1] = (int)((begin - at) / t);
-                found[2] = (int)((begin - at) % t);
-                break;
-            }
-            at += (int64_t)t * R;
-        }
-    }
-    __syncthreads();
     PaCursor ld, cp;
-    ld.b = found[0];
-    ld.r = found[1];
-    ld.tile = found[2];
-    ld.len = clamp_len(__ldg(p.lens + ld.b), p.cap);
-    ld.tiles = tiles_of(ld.len);
+    int64_t total, blocks, begin, end;
+    if (p.whole_rows) {  // few short rows: a block each, nothing to join
+        ld.b = blockIdx.x / R;
+        ld.r = blockIdx.x % R;
+        ld.tile = 0;
+        ld.len = clamp_len(__ldg(p.lens + ld.b), p.cap);
+        ld.tiles = tiles_of(ld.len);
+        total = end = ld.tiles;
+        blocks = 1;
+        begin = 0;
+    } else {
+        int64_t *scan = reinterpret_cast<int64_t *>(smem_pa + Cfg::kOffScan);  // [4] warp sums
+        int *found = reinterpret_cast<int *>(scan + 4);                        // b, r, tile
+        const int per = (p.B + kThreads - 1) / kThreads;
+        const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
+        int64_t mine = 0;
+        for (int b = b0; b < b1; ++b) mine += tiles_of(clamp_len(__ldg(p.lens + b), p.cap));
+        mine *= R;
+        int64_t incl = mine;
+#pragma unroll
+        for (int s = 1; s < 32; s <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, incl, s);
+            if (lane >= s) incl += up;
+        }
+        if (lane == 31) scan[warp] = incl;
+        __syncthreads();
+        int64_t excl = incl - mine;
+        total = 0;
+#pragma unroll
+        for (int w = 0; w < kPaWarps; ++w) {
+            if (w < warp) excl += scan[w];
+            total += scan[w];
+        }
+        blocks = min64(gridDim.x, total);  // none of them without a tile
+        if (blockIdx.x >= blocks) return;
+        begin = total * blockIdx.x / blocks;
+        end = total * (blockIdx.x + 1) / blocks;
+        if (begin >= excl && begin < excl + mine) {
+            int64_t at = excl;
+            for (int b = b0; b < b1; ++b) {
+                const int t = tiles_of(clamp_len(__ldg(p.lens + b), p.cap));
+                if (begin < at + (int64_t)t * R) {
+                    found[0] = b;
+                    found[1] = (int)((begin - at) / t);
+                    found[2] = (int)((begin - at) % t);
+                    break;
+                }
+                at += (int64_t)t * R;
+            }
+        }
+        __syncthreads();
+        ld.b = found[0];
+        ld.r = found[1];
+        ld.tile = found[2];
+        ld.len = clamp_len(__ldg(p.lens + ld.b), p.cap);
+        ld.tiles = tiles_of(ld.len);
+    }
     cp = ld;
     int64_t row_begin = begin - cp.tile;  // first tile of the current row, in the total
 
@@ -643,7 +658,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
             if (it + 1 < n_tiles) stage_q();
             const bool first = row_start_tile == row_begin, whole = first && last;
             const int part = blockIdx.x * 2 + (first ? 1 : 0);
-            if (first && tid == 0) {
+            if (first && tid == 0 && !p.whole_rows) {
                 // the block that holds tile t of the total is floor(((t + 1) * blocks - 1) / total)
                 const int64_t t = row_begin + row_tiles - 1;
                 p.parts[done.b * R + done.r] = make_int2((int)blockIdx.x, (int)(((t + 1) * blocks - 1) / total));

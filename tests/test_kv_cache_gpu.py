@@ -119,6 +119,22 @@ def test_attention_over_long_and_many_sequences(gae, dtype, B, H, Hkv, D, n):
     _check_attention(gae, q, k, v, table, lens, weights=w)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("cap", [64, 192, 193, 384, 385])
+def test_attention_of_short_rows(gae, dtype, cap):
+    """Tables around the longest row that one block takes whole, few rows and more rows than blocks."""
+    for B, H, Hkv, D in ((5, 6, 2, 128), (120, 20, 5, 64)):
+        g = _gen(cap + B)
+        k, v = _pools(B * cap // 8 + 9, Hkv, 8, D, dtype, g)
+        M = -(-cap // 8)
+        table = _table(B, M, k.shape[0], g) if B * M <= k.shape[0] else \
+            torch.randint(0, k.shape[0], (B, M), device="cuda", generator=g, dtype=torch.int32)
+        q = torch.randn(B, H, D, device="cuda", generator=g).to(dtype)
+        lens = torch.tensor([(b * 67 + 11) % (cap + 2) for b in range(B)], dtype=torch.int32, device="cuda")
+        lens[0] = 0
+        _check_attention(gae, q, k, v, table, lens)
+
+
 def test_attention_passes_over_pages_that_hold_nothing(gae):
     g, B, Hkv, page, D = _gen(3), 4, 2, 16, 128
     k, v = _pools(40, Hkv, page, D, torch.bfloat16, g)
