@@ -82,8 +82,8 @@ PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool
 // How many CTAs share a pair of key tiles' queries: enough to fill the GPU (two
 // CTAs to an SM) as long as each is left with 4 query tiles (1000 x 1000, 24
 // heads x 64: 12.5 us replayed from a graph with 4, 12.7 with 2, 15.9 with 8 and
-// thus one launch).  (Four times as many, so that a causal mask's long units end together, gained nothing: 178
-// against 180 us at 8192 x 8192, 16 heads.)
+// thus one launch).  (Four times as many, so that a causal mask's long units end
+// together, gained nothing: 178 against 180 us at 8192 x 8192, 16 heads.)
 int key_weights_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nkv) {
     const int64_t units = B * Hkv * ((Nkv + 255) / 256), tiles = H / Hkv * ((Nq + 127) / 128);
     return (int)gae::max64(1, gae::min64((2 * num_sms() + units - 1) / units, tiles / 4));
@@ -125,7 +125,7 @@ gae_status launch_paged_attn(gae::PagedAttnParams p, cudaStream_t st) {
     if ((s = set_smem(gae::paged_attn_kernel<Tile, DM>, Cfg::kSmem)) != GAE_OK) return s;
     p.groups = (p.G + Tile::kHeads - 1) / Tile::kHeads;
     const int64_t rows = (int64_t)p.B * p.pool.Hkv * p.groups;
-    const int tile_keys = gae::kPaWarps * Tile::kKeys;
+    constexpr int tile_keys = Cfg::kTileKeys;
     const int64_t most = rows * gae::max64(1, (p.cap + tile_keys - 1) / tile_keys);
     const int64_t slots = (int64_t)num_sms() * Cfg::kPerSm;
     // Rows of up to 6 tiles are left whole where each has a block at once: one
@@ -133,7 +133,7 @@ gae_status launch_paged_attn(gae::PagedAttnParams p, cudaStream_t st) {
     // a graph, 16.5 against 18.7 a call from Python; 8 tiles: 7.6 against 6.3.
     p.whole_rows = !p.scores && p.cap <= 6 * tile_keys && rows <= slots;
     const unsigned blocks = (unsigned)(p.whole_rows ? rows : gae::min64(most, slots));
-    gae::paged_attn_kernel<Tile, DM><<<blocks, gae::kPaWarps * 32, Cfg::kSmem, st>>>(p);
+    gae::paged_attn_kernel<Tile, DM><<<blocks, Cfg::kThreads, Cfg::kSmem, st>>>(p);
     GAE_CUDA_TRY(cudaGetLastError());
     if (p.whole_rows || (p.cap <= tile_keys && !p.scores)) return GAE_OK;  // nothing was split
     const int64_t chunks = p.scores ? gae::min64((p.cap + gae::kJoinKeys - 1) / gae::kJoinKeys, 32768) : 0;

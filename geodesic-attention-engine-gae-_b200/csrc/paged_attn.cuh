@@ -6,13 +6,13 @@
 // Every cached row is read once for all query heads that share it, so the work
 // is bound by the cache's bytes; the kernels are built to keep enough of them
 // in flight.  A row (sequence, key head, group of up to 16 query heads) is cut
-// into tiles of kKeys * 4 positions and the tiles of all rows, in order, are
+// into tiles of kKeys positions to a warp and the tiles of all rows, in order, are
 // dealt in equal runs to a grid that fills the GPU once, whatever the lengths
 // are: they are read on the device, so a captured graph stays balanced when
 // they change.  A block that ends inside a row leaves (max, sum, O) of its part
 // in the workspace; paged_attn_join_kernel adds those parts in a fixed order.
 //
-// Inside a block the four warps take 16 rows (8 for fp32) of each tile each,
+// Inside a block the warps take 16 rows (8 for fp32) of each tile each,
 // with their own ring of cp.async stages, maximum, sum and accumulator: nothing
 // is shared until the row ends, so no barrier stands between tiles.
 //
@@ -23,7 +23,9 @@
 // pass over 8.4 MB of scores is latency: 10 us).  What made it so: three blocks
 // of two stages to an SM over two of three (172 against 180 us at the first
 // size), the next tile's loads before this tile's products, the next row's q
-// before the merge, and one page look-up to a tile (all four: 262 to 172 us).
+// before the merge, and one page look-up to a tile (all four: 262 to 172 us).  At
+// head_dim 256 six warps to a block: 16 x 16 heads, up to 4096 positions, bf16,
+// 95 us, 103 with four.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -56,7 +58,6 @@ struct PagedAttnParams {
     float *part_o;        // [blocks][2][heads of a tile][D]
 };
 
-constexpr int kPaWarps = 4;
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool pred) {
@@ -379,14 +380,17 @@ struct PaFmaTile {
 template <class Tile, int DM>
 struct PaCfg {
     static constexpr int kSlot = Tile::kKeys * DM * (int)sizeof(typename Tile::Elem) * 2;  // K and V rows of a warp
+    // Two stages and as many warps as the shared memory feeds: three blocks of
+    // four, or at head_dim 256 one of six.
+    static constexpr int kWarps = DM == 256 ? 6 : 4, kThreads = kWarps * 32, kTileKeys = kWarps * Tile::kKeys;
     static constexpr int kStages = DM == 64 ? 4 : 2;
-    static constexpr int kRing = kPaWarps * kStages * kSlot;
+    static constexpr int kRing = kWarps * kStages * kSlot;
     static constexpr int kOffMl = kRing;                                   // [warps][heads][2]
-    static constexpr int kOffQ = kOffMl + kPaWarps * Tile::kHeads * 8;     // fp32 tiles: q [heads][DM]
+    static constexpr int kOffQ = kOffMl + kWarps * Tile::kHeads * 8;     // fp32 tiles: q [heads][DM]
     static constexpr bool kQ = sizeof(typename Tile::Elem) == 4;
     static constexpr int kOffP = kOffQ + (kQ ? Tile::kHeads * DM * 4 : 0);  // fp32 tiles: probabilities
-    static constexpr int kOffValid = kOffP + kPaWarps * Tile::kWarpScratch * 4;
-    static constexpr int kOffScan = kOffValid + kPaWarps * kStages * 4;
+    static constexpr int kOffValid = kOffP + kWarps * Tile::kWarpScratch * 4;
+    static constexpr int kOffScan = kOffValid + kWarps * kStages * 4;
     static constexpr int kSmem = (kOffScan + 64 + 15) / 16 * 16;
     static constexpr int kPerSm = 3 * (kSmem + 1024) <= 228 * 1024 ? 3 : 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;
     // the merge reuses a stage: fp32 [heads][DM]
@@ -400,10 +404,10 @@ struct PaCursor {
 };
 
 template <class Tile, int DM>
-__global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(PaCfg<Tile, DM>::kThreads, PaCfg<Tile, DM>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     using Cfg = PaCfg<Tile, DM>;
     using T = typename Tile::Elem;
-    constexpr int kKeys = Tile::kKeys, kTileKeys = kPaWarps * kKeys, kThreads = kPaWarps * 32;
+    constexpr int kKeys = Tile::kKeys, kWarps = Cfg::kWarps, kTileKeys = Cfg::kTileKeys, kThreads = Cfg::kThreads;
     extern __shared__ __align__(128) uint8_t smem_pa[];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int R = p.pool.Hkv * p.groups;  // rows of a sequence
@@ -424,7 +428,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
         blocks = 1;
         begin = 0;
     } else {
-        int64_t *scan = reinterpret_cast<int64_t *>(smem_pa + Cfg::kOffScan);  // [4] warp sums
+        int64_t *scan = reinterpret_cast<int64_t *>(smem_pa + Cfg::kOffScan);  // [kWarps] warp sums
         int *found = reinterpret_cast<int *>(scan + 4);                        // b, r, tile
         const int per = (p.B + kThreads - 1) / kThreads;
         const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
@@ -442,7 +446,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
         int64_t excl = incl - mine;
         total = 0;
 #pragma unroll
-        for (int w = 0; w < kPaWarps; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
             if (w < warp) excl += scan[w];
             total += scan[w];
         }
@@ -637,7 +641,7 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
         __syncwarp();
         const bool last = cp.tile + 1 == cp.tiles;
         if (last || it + 1 == n_tiles) {
-            // --- the row's end here: the four warps' parts become one.  The next
+            // --- the row's end here: the warps' parts become one.  The next
             // row's q is on its way meanwhile.
             const Row done = row;
             const int row_tiles = cp.tiles;
@@ -665,16 +669,16 @@ __global__ void __launch_bounds__(kPaWarps * 32, PaCfg<Tile, DM>::kPerSm) paged_
             }
             for (int i = tid; i < done.heads * (DM / 4); i += kThreads) {
                 const int h = i / (DM / 4), d = i % (DM / 4) * 4;
-                float mw[kPaWarps], mx = -INFINITY, l = 0.f;
+                float mw[kWarps], mx = -INFINITY, l = 0.f;
 #pragma unroll
-                for (int w = 0; w < kPaWarps; ++w) {
+                for (int w = 0; w < kWarps; ++w) {
                     mw[w] = sml[(w * Tile::kHeads + h) * 2];
                     mx = fmaxf(mx, mw[w]);
                 }
                 const float base = mx == -INFINITY ? 0.f : mx;
                 float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kPaWarps; ++w) {
+                for (int w = 0; w < kWarps; ++w) {
                     const float f = ex2_approx(mw[w] - base);
                     l += f * sml[(w * Tile::kHeads + h) * 2 + 1];
                     const float4 x = *reinterpret_cast<const float4 *>(
