@@ -391,7 +391,7 @@ struct PaCfg {
     static constexpr int kOffP = kOffQ + (kQ ? Tile::kHeads * DM * 4 : 0);  // fp32 tiles: probabilities
     static constexpr int kOffValid = kOffP + kWarps * Tile::kWarpScratch * 4;
     static constexpr int kOffScan = kOffValid + kWarps * kStages * 4;
-    static constexpr int kSmem = (kOffScan + 64 + 15) / 16 * 16;
+    static constexpr int kSmem = (kOffScan + kWarps * 8 + 16 + 15) / 16 * 16;
     static constexpr int kPerSm = 3 * (kSmem + 1024) <= 228 * 1024 ? 3 : 2 * (kSmem + 1024) <= 228 * 1024 ? 2 : 1;
     // the merge reuses a stage: fp32 [heads][DM]
     static_assert(Tile::kHeads * DM * 4 <= kSlot, "a warp's O has to fit its stage");
@@ -404,7 +404,8 @@ struct PaCursor {
 };
 
 template <class Tile, int DM>
-__global__ void __launch_bounds__(PaCfg<Tile, DM>::kThreads, PaCfg<Tile, DM>::kPerSm) paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
+__global__ void __launch_bounds__(PaCfg<Tile, DM>::kThreads, PaCfg<Tile, DM>::kPerSm)
+    paged_attn_kernel(const __grid_constant__ PagedAttnParams p) {
     using Cfg = PaCfg<Tile, DM>;
     using T = typename Tile::Elem;
     constexpr int kKeys = Tile::kKeys, kWarps = Cfg::kWarps, kTileKeys = Cfg::kTileKeys, kThreads = Cfg::kThreads;
@@ -429,7 +430,7 @@ __global__ void __launch_bounds__(PaCfg<Tile, DM>::kThreads, PaCfg<Tile, DM>::kP
         begin = 0;
     } else {
         int64_t *scan = reinterpret_cast<int64_t *>(smem_pa + Cfg::kOffScan);  // [kWarps] warp sums
-        int *found = reinterpret_cast<int *>(scan + 4);                        // b, r, tile
+        int *found = reinterpret_cast<int *>(scan + kWarps);                   // b, r, tile
         const int per = (p.B + kThreads - 1) / kThreads;
         const int b0 = min(p.B, tid * per), b1 = min(p.B, b0 + per);
         int64_t mine = 0;
