@@ -70,8 +70,8 @@ struct AppendParams {
 };
 
 // A thread copies 16 bytes of kAppendRows new rows, K and V both; all of its
-// reads are on their way before it writes (one row to a thread keeps a 335 MB
-// prompt at 66 us, four bring it to the copy rate).
+// reads are on their way before it writes.  Bound by memory: 335 MB of a prompt
+// read and written take 57 us (89% of the copy rate), 66 with one row to a thread.
 constexpr int kAppendRows = 4;
 
 template <int ESIZE>

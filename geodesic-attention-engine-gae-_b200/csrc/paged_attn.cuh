@@ -694,7 +694,8 @@ __global__ void __launch_bounds__(PaCfg<Tile, DM>::kThreads, PaCfg<Tile, DM>::kP
                     if constexpr (sizeof(T) == 4) {
                         *reinterpret_cast<float4 *>(o) = make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
                     } else {
-                        T v[4] = {from_f<T>(acc.x * inv), from_f<T>(acc.y * inv), from_f<T>(acc.z * inv), from_f<T>(acc.w * inv)};
+                        alignas(8) T v[4] = {from_f<T>(acc.x * inv), from_f<T>(acc.y * inv), from_f<T>(acc.z * inv),
+                                             from_f<T>(acc.w * inv)};
                         *reinterpret_cast<uint2 *>(o) = *reinterpret_cast<const uint2 *>(v);
                     }
                     if (d == 0) {
@@ -721,10 +722,11 @@ __global__ void __launch_bounds__(PaCfg<Tile, DM>::kThreads, PaCfg<Tile, DM>::kP
 }
 
 // Joins the parts of rows that more than one block worked on: block (row, y), y
-// < join_heads, joins head y; further blocks of the row's key head add up
-// the keys' weights, kJoinKeys positions at a time (512 to 2048 measure alike).
-// The kernel is all latency: every thread reads its parts' statistics and sums side by side and scales as
-// it goes, so that one trip to memory follows the row's entry in `parts`.
+// < join_heads, joins head y; further blocks of the row's key head add up the
+// keys' weights, kJoinKeys positions at a time (512 to 2048 measure alike).  The
+// kernel is all latency: every thread reads its parts' statistics and sums side by
+// side and scales as it goes, so that one trip to memory follows the row's entry
+// in `parts`.
 constexpr int kJoinThreads = 256, kJoinKeys = 1024;
 
 // (m, l) and (m2, l2), sums relative to 2^m, become one; f and f2 scale what
@@ -738,7 +740,8 @@ __device__ __forceinline__ void join_sums(float &m, float &l, float m2, float l2
 }
 
 template <typename T>
-__global__ void __launch_bounds__(kJoinThreads) paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p, int tile_heads, int join_heads) {
+__global__ void __launch_bounds__(kJoinThreads)
+    paged_attn_join_kernel(const __grid_constant__ PagedAttnParams p, int tile_heads, int join_heads) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int R = p.pool.Hkv * p.groups, row = blockIdx.x, b = row / R, r = row % R, D = p.pool.D;
     const int hk = r / p.groups, tid = threadIdx.x;
