@@ -18,9 +18,11 @@
 //
 // What bounds it: one exponential per score.  The MUFU gives 16 a cycle and
 // SM, a 128 x 128 tile takes it 1024 cycles where the products at head_dim 128
-// take 512; every kKwPolyPeriod-th pair therefore goes to a polynomial on the
-// FMA pipe.
+// take 512.  All exponentials are the MUFU's, which keeps NaN, gives +inf from
+// 2^128 on and 0 below 2^-126 whatever column a query stands in.
 #pragma once
+#include <cfloat>
+
 #include "attn_bwd_sm100.cuh"
 #include "sm100.cuh"
 
@@ -41,36 +43,6 @@ enum KeyWeightsWaitSite : unsigned {
     kSiteKwK = 0x501, kSiteKwQFull = 0x502, kSiteKwQEmpty = 0x503, kSiteKwS = 0x504, kSiteKwSEmpty = 0x505,
     kSiteKwDone = 0x506, kSiteKwSmem = 0x507,
 };
-
-constexpr int kKwPolyPeriod = 3;
-
-// 2^x for a pair of x <= 2^22 on the FMA pipe: exp2_poly_x2's range reduction
-// with a polynomial of degree 5, whose coefficients are the minimax fit of 2^f
-// on [0, 1) in relative error (by linear programming over 4001 points; max
-// relative error 7.5e-8, 1.5e-7 in fp32), as exact as the MUFU's 2^-22.  Results
-// below 2^-126 come out as 2^-126.
-__device__ __forceinline__ uint64_t exp2_poly5_x2(uint64_t x2) {
-    constexpr float kMagic = 12582912.0f;  // 1.5 * 2^23
-    float x0, x1;
-    f2_unpack(x2, x0, x1);
-    const uint64_t xc = f2_pack(fmaxf(x0, -126.f), fmaxf(x1, -126.f));
-    const uint64_t mg = f2_pack(kMagic, kMagic);
-    uint64_t t, j, f;
-    asm("add.rm.f32x2 %0, %1, %2;" : "=l"(t) : "l"(xc), "l"(mg));
-    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(j) : "l"(t), "l"(mg));
-    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(f) : "l"(xc), "l"(j));
-    uint64_t p = f2_fma(f, f2_pack(0.00187757204f, 0.00187757204f), f2_pack(0.00898935273f, 0.00898935273f));
-    p = f2_fma(p, f, f2_pack(0.0558263063f, 0.0558263063f));
-    p = f2_fma(p, f, f2_pack(0.240153626f, 0.240153626f));
-    p = f2_fma(p, f, f2_pack(0.693153083f, 0.693153083f));
-    p = f2_fma(p, f, f2_pack(0.99999994f, 0.99999994f));
-    float p0, p1, t0, t1;
-    f2_unpack(p, p0, p1);
-    f2_unpack(t, t0, t1);
-    // bits(t) * 2^23 puts j into the exponent field; adding bits(p) scales p by 2^j
-    return f2_pack(__uint_as_float(__float_as_uint(t0) * 8388608u + __float_as_uint(p0)),
-                   __uint_as_float(__float_as_uint(t1) * 8388608u + __float_as_uint(p1)));
-}
 
 template <int D>
 struct KeyWeightsCfg {
@@ -108,6 +80,7 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Cfg::kOffBar + Cfg::kNumBars * 8);
     volatile int *abort_flag = reinterpret_cast<volatile int *>(tmem_slot + 1);
     volatile int no_abort = 0;
+    volatile int *s_none = reinterpret_cast<volatile int *>(tmem_slot + 2);  // [2] a query of the tile saw no key
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
@@ -196,15 +169,19 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             mbar_wait(bar_done, 0, kSiteKwDone, &no_abort);
         }
     } else if (warp == Cfg::kLseWarp) {
-        // -lse of the tile's queries in log2; -inf where the row saw no key.  Two
-        // buffers: warpgroups that have let go of S tile it - 1 are done with tile
-        // it - 2.
+        // -lse of the tile's queries in log2.  +inf marks a row that saw no key
+        // (lse = -inf) or does not exist: its weights are 0 whatever its scores,
+        // and s_none sends its tile to the epilogue's selecting path.  A finite
+        // lse whose negative passes fp32's range stays finite: no mark.  Two
+        // buffers: warpgroups that have let go of S tile it - 1 are done with
+        // tile it - 2.
         auto fetch = [&](float (&v)[4]) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int r = (i0 + i) * 128 + e * 32 + lane;
                 const float l = r < p.Nq ? __ldg(p.lse + b * p.l_sb + h * p.l_sh + r) : -INFINITY;
-                v[e] = l == -INFINITY ? -INFINITY : -l * 1.4426950408889634f;
+                v[e] = -l * 1.4426950408889634f;
+                if (v[e] == INFINITY && l != -INFINITY) v[e] = FLT_MAX;
             }
             next_tile();
         };
@@ -217,6 +194,8 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             if (!ok) break;
 #pragma unroll
             for (int e = 0; e < 4; ++e) s_lse[(it & 1) * 128 + e * 32 + lane] = v[e];
+            const int none = __any_sync(0xffffffffu, fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3])) == INFINITY);
+            if (lane == 0) s_none[it & 1] = none;
             if (it + 1 < n_it) fetch(v);
             for (int kt = 0; kt < n_kt; ++kt) mbar_arrive(bar_s_full(kt));
         }
@@ -239,7 +218,8 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
             tc_fence_after();
             const uint32_t sl = base + Cfg::kOffLse + (it & 1) * 512;
             uint64_t acc[4] = {};
-            if (first_high <= q0 && q0 + 128 <= p.Nq) {  // every key of the warp is seen by all 128 queries
+            // every key of the warp is seen by all 128 queries, each of which saw one
+            if (first_high <= q0 && !s_none[it & 1]) {
 #pragma unroll
                 for (int c0 = 0; c0 < 128; c0 += 32) {
                     uint32_t r[32];
@@ -256,24 +236,18 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
 #pragma unroll
                         for (int u = 0; u < 2; ++u) {
                             const int c = 2 * (e + u);
-                            const uint64_t x =
-                                f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, n[u]);
-                            uint64_t w;
-                            if ((e + u) % kKwPolyPeriod == kKwPolyPeriod - 1) {
-                                w = exp2_poly5_x2(x);
-                            } else {
-                                float x0, x1;
-                                f2_unpack(x, x0, x1);
-                                w = f2_pack(ex2_approx(x0), ex2_approx(x1));
-                            }
+                            float x0, x1;
+                            f2_unpack(f2_fma(f2_pack(__uint_as_float(r[c]), __uint_as_float(r[c + 1])), sl2, n[u]), x0, x1);
+                            const uint64_t w = f2_pack(ex2_approx(x0), ex2_approx(x1));
                             acc[(e + u) & 3] = f2_add(acc[(e + u) & 3], w);
                         }
                     }
                 }
             } else {
-                // Columns [lo, hi) count; those from hi on are no queries (their rows
-                // are zeros: a NaN key would reach the sum).  32 columns that no key
-                // of the warp counts are passed over.
+                // Columns [lo, hi) count (from hi on there are no queries), but for
+                // those marked as having seen no key: a select, since their scores
+                // may be NaN or infinite.  32 columns that no key of the warp counts
+                // are passed over.
                 const int lo = first - q0, hi = min(128, p.Nq - q0);
 #pragma unroll 1
                 for (int c0 = max(0, first_low - q0) & ~31; c0 < hi; c0 += 32) {
@@ -285,10 +259,11 @@ __global__ void __launch_bounds__(KeyWeightsCfg<D>::kThreads, 2)
                         uint64_t n0;
                         asm volatile("ld.shared.b64 %0, [%1];" : "=l"(n0) : "r"(sl + c0 * 4 + e * 8));
                         const int c = c0 + 2 * e;
-                        float x0, x1;
+                        float x0, x1, l0, l1;
                         f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), sl2, n0), x0, x1);
-                        const float w0 = c >= lo && c < hi ? ex2_approx(x0) : 0.f;
-                        const float w1 = c + 1 >= lo && c + 1 < hi ? ex2_approx(x1) : 0.f;
+                        f2_unpack(n0, l0, l1);
+                        const float w0 = c >= lo && l0 != INFINITY ? ex2_approx(x0) : 0.f;
+                        const float w1 = c + 1 >= lo && l1 != INFINITY ? ex2_approx(x1) : 0.f;
                         acc[e & 3] = f2_add(acc[e & 3], f2_pack(w0, w1));
                     }
                 }

@@ -660,3 +660,76 @@ def test_decoding_step_in_a_graph(gae):
     assert graphed.lengths != [steps] * B  # the host has not seen the replays
     graphed.refresh()
     assert graphed.lengths == graphed.lens.tolist() == [steps] * B
+
+
+# What key weights are made of, in tiles of 128 queries that every key sees and in the others: 384 queries, of which
+# the third tile is cut by the mask, against 256 keys (causal: query row r sees key c iff c <= r + 128).
+def _full_tiles(seed, dtype=torch.bfloat16, D=64):
+    g = _gen(seed)
+    q = torch.randn(1, 2, 384, D, device="cuda", generator=g).to(dtype)
+    k = torch.randn(1, 1, 256, D, device="cuda", generator=g).to(dtype)
+    return q, k, torch.full((1, 2, 384), 6.0, device="cuda")
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_key_weights_of_queries_that_saw_nothing_are_nothing(gae, dtype, causal):
+    """A query whose lse is -inf adds exactly nothing, whatever it holds and wherever it stands: the
+    other queries' weights are the same bits, keys that only such queries see have a weight of 0."""
+    q, k, lse = _full_tiles(40, dtype)
+    kw = dict(causal=causal, q_offset=128 if causal else 0)
+    assert (gae.attention_key_weights(q, k, torch.full_like(lse, -math.inf), **kw) == 0).all()
+    out = torch.arange(lse.shape[2], device="cuda") % 7 == 3  # rows of every tile, and all of the last one
+    out[256:] = True
+    lse[:, :, out] = -math.inf
+    want = gae.attention_key_weights(q, k, lse, **kw)
+    _check_keys(gae, q, k, lse, want, causal, kw["q_offset"])
+    for junk in (math.nan, math.inf, -math.inf, 0.0):
+        q2 = q.clone()
+        q2[:, :, out] = junk
+        assert torch.equal(gae.attention_key_weights(q2, k, lse, **kw), want), junk
+
+
+def test_key_weights_of_a_nan_query_are_nan_at_every_column(gae):
+    """A NaN query (its lse is NaN too) makes every key that sees it NaN, in whole tiles and cut ones alike."""
+    q, k, lse = _full_tiles(41)
+    for row in range(256):
+        q2, l2 = q.clone(), lse.clone()
+        q2[0, 1, row], l2[0, 1, row] = math.nan, math.nan
+        w = gae.attention_key_weights(q2, k, l2)
+        assert w.isnan().all(), row
+        w = gae.attention_key_weights(q2, k, l2, causal=True, q_offset=128)
+        seen = torch.arange(256, device="cuda") <= row + 128
+        assert w[0, 0, seen].isnan().all() and w[0, 0, ~seen].isfinite().all(), row
+        w = gae.attention_key_weights(q2, k, lse)  # a NaN query whose lse is finite
+        assert w.isnan().all(), row
+
+
+@pytest.mark.parametrize("row", [0, 1, 2, 3, 4, 5, 30, 31, 100, 127, 128, 300, 383])
+def test_key_weights_of_scores_far_above_the_lse(gae, row):
+    """An lse that does not cover the keys (a part's, before a merge): weights as large as fp32 has them,
+    then +inf, from any column.  fp32 ends at e^88.72."""
+    q, k, lse = _full_tiles(42)
+    q.zero_()  # every score is 0: a weight is exp(-lse)
+    for l, want in ((-87.0, math.exp(87.0)), (-88.5, math.exp(88.5)), (-89.0, math.inf), (-97.0, math.inf),
+                    (-150.0, math.inf), (-3e38, math.inf)):
+        l2 = lse.clone()
+        l2[0, 0, row] = l
+        w = gae.attention_key_weights(q, k, l2).double()
+        # the exponent's argument is off by 4 u |lse| at most, the exponential by 2^-20
+        assert (w == want).all() if want == math.inf else ((w / want - 1).abs() <= 4 * U * 90 + 2.0 ** -20).all(), l
+    l2 = lse.clone()
+    l2[0, 0, row] = math.inf  # a row that saw an infinite score: exp(-inf)
+    others = torch.ones(384, dtype=torch.bool, device="cuda")
+    others[row] = False
+    want = 2 * 384 * math.exp(-6.0) - math.exp(-6.0)
+    w = gae.attention_key_weights(q, k, l2).double()
+    assert ((w / want - 1).abs() <= 4 * U * 6 + 2.0 ** -20 + 768 * U).all()
+
+
+def test_key_weights_of_far_scores_are_nothing(gae):
+    """Weights below fp32's smallest normal number come out as 0, from any column."""
+    q, k, lse = _full_tiles(43)
+    q.zero_()
+    lse.fill_(104.0)
+    assert (gae.attention_key_weights(q, k, lse) == 0).all()
