@@ -390,7 +390,9 @@ gae_status gae_paged_evict(const gae_kv_pool *pool, const gae_paged_evict_args *
     const int max_keys = (int)gae::min64(((p.cap + cluster - 1) / cluster + 3) / 4 * 4, gae::kEvictMaxKeys);
     if (rows * cluster > INT32_MAX) return fail(GAE_ERR_UNSUPPORTED, "too many rows");
     const int smem = (2 * gae::kEvictBins + max_keys) * 4;
-    if ((s = set_smem(gae::evict_select_kernel, smem)) != GAE_OK) return s;
+    // The limit belongs to the kernel, not to this call: always the largest, so
+    // that no other thread's call lowers it between here and the launch.
+    if ((s = set_smem(gae::evict_select_kernel, (2 * gae::kEvictBins + gae::kEvictMaxKeys) * 4)) != GAE_OK) return s;
     cudaLaunchConfig_t cfg;
     memset(&cfg, 0, sizeof(cfg));
     cfg.gridDim = dim3((unsigned)(rows * cluster));

@@ -11,7 +11,9 @@ terms, the exponential's own 2 units in the last place on either side), and
 output is a mean of V under them: off by that share of max |V|, and by half a
 step of its own type, eps / 2 of the value.  The log-sum-exp is off by that
 share plus its own rounding."""
+import ctypes
 import math
+import threading
 
 import pytest
 
@@ -733,3 +735,39 @@ def test_key_weights_of_far_scores_are_nothing(gae):
     q.zero_()
     lse.fill_(104.0)
     assert (gae.attention_key_weights(q, k, lse) == 0).all()
+
+
+def test_evict_from_host_threads(gae):
+    """Caches of very different lengths evicted at the same time through the C entry, by a thread and on a
+    stream each: no call may lose its launch to another's."""
+    g, page, D, turns = _gen(45), 16, 64, 3000
+    cases = []
+    for n, keep in ((500, 20), (39_000, 20)) * 3:
+        M = (n + page - 1) // page
+        k, v = _pools(M + 2, 1, page, D, torch.bfloat16, g)
+        both = _table(1, M + 2, M + 2, g)
+        w = torch.rand(1, 1, n, device="cuda", generator=g)
+        lens = torch.tensor([n], dtype=torch.int32, device="cuda")
+        new, kept = torch.zeros_like(lens), torch.zeros(1, 1, keep, dtype=torch.int32, device="cuda")
+        kw = torch.zeros(1, 1, keep, device="cuda")
+        pool = gae.KvPool(k.data_ptr(), v.data_ptr(), tuple(k.stride()[:3]), tuple(v.stride()[:3]), *k.shape, gae.DTYPE_BF16)
+        args = gae.PagedEvictArgs(1, both.data_ptr(), M + 2, M, lens.data_ptr(), w.data_ptr(), (n, n), n,
+                                  both.data_ptr() + 4 * M, M + 2, 2, keep, 0, new.data_ptr(), kept.data_ptr(), kw.data_ptr())
+        want = torch.sort(w[0, 0], descending=True, stable=True).indices[:keep].sort().values
+        cases.append((pool, args, torch.cuda.Stream(), kept, want, (k, v, both, w, lens, new, kw)))
+    torch.cuda.synchronize()
+    L, status = gae.lib(), []
+
+    def work(pool, args, stream):
+        st = stream.cuda_stream
+        status.extend({L.gae_paged_evict(ctypes.byref(pool), ctypes.byref(args), st) for _ in range(turns)})
+
+    threads = [threading.Thread(target=work, args=c[:3]) for c in cases]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert status == [0] * len(cases)
+    for c in cases:
+        assert torch.equal(c[3][0, 0].long(), c[4])
