@@ -95,8 +95,8 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
             : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// How far a score may pass the exponent's base before the accumulator is
-// rescaled: probabilities stay below 2^8, well inside f16.
+// How far a score may pass the maximum so far (log2) before the accumulator is
+// rescaled.
 constexpr float kPaSlack = 8.f;
 
 // 16 cached rows against up to NT * 8 query heads on the tensor cores, keys as
@@ -111,11 +111,17 @@ template <typename T, int DM, int NT>
 struct PaMmaTile {
     static constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
     static constexpr int kHeads = NT * 8, kKeys = 16, kChunks = DM * 2 / 16;
+    // f16 probabilities are held times 2^13, so that they end where f16 does: the
+    // largest lies in [2^13, 2^15], and the steps of 2^-24 at f16's lower end are
+    // 2^-37 of it (from 2^-24 of it on they would round to nothing: of 131072 keys,
+    // 2^-24 as heavy as the heaviest each, that is 2^-7 of the output).
+    static constexpr float kSlack = kBF16 ? kPaSlack : 2.f, kUp = kBF16 ? 0.f : 13.f;
     static constexpr int kWarpScratch = 0;
     using Elem = T;
     __device__ explicit PaMmaTile(const float *) {}
     uint32_t qf[NT][DM / 16][2];
-    float o[NT][DM / 16][4], m[NT][2], l[NT][2];
+    float o[NT][DM / 16][4], l[NT][2];
+    float m[NT][2];  // the exponents' base: kUp below the maximum that it was last set by
 
     // Shared-memory byte offset of 16-byte chunk c of row r (ldmatrix reads 8
     // rows of one chunk: the swizzle puts them in different banks).
@@ -174,7 +180,7 @@ struct PaMmaTile {
                     if (h < heads) scores[(int64_t)(r + 8 * (e >> 1)) * G + h] = v;
                 }
                 x[n][e] = ok[e >> 1] ? v : -INFINITY;
-                grow |= x[n][e] > m[n][e & 1] + kPaSlack;
+                grow |= x[n][e] > m[n][e & 1] + (kUp + kSlack);
             }
         if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -184,7 +190,7 @@ struct PaMmaTile {
                     float mx = fmaxf(x[n][e], x[n][e + 2]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-                    mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)), m[n][e]);
+                    mx = fmaxf(fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16)) - kUp, m[n][e]);
                     const float alpha = m[n][e] == -INFINITY ? 0.f : ex2_approx(m[n][e] - mx);
                     m[n][e] = mx;
                     l[n][e] *= alpha;

@@ -771,3 +771,31 @@ def test_evict_from_host_threads(gae):
     assert status == [0] * len(cases)
     for c in cases:
         assert torch.equal(c[3][0, 0].long(), c[4])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("below", [14, 20, 24, 28])
+def test_attention_of_many_light_keys_beside_heavy_ones(gae, dtype, below):
+    """Four keys of the first 64 take nearly all of each probability and their value is 0: the output is the
+    sum of very many small probabilities, 2^-below of a heavy key's each.  No term is negative, so the
+    file's share holds of the output itself; a f16 probability is besides off by 2^-38 of the heaviest at
+    most.  So many rows (of the same pages) that a block has whole ones."""
+    B, n, D, page = 888, 131072, 64, 64
+    g = _gen(44 + below)
+    k, v = _pools(n // page, 1, page, D, dtype, g)
+    k.zero_()
+    v.abs_()
+    table = _table(1, n // page, n // page, g)
+    at = table[0, 0].long()
+    k[at, 0, 5::16, 0], v[at, 0, 5::16] = 1.0, 0.0
+    q = torch.zeros(1, 2, D, device="cuda", dtype=dtype)
+    q[0, :, 0] = below + torch.tensor([0.5, 0.25], device="cuda")
+    lens = torch.full((B,), n, dtype=torch.int32, device="cuda")
+    out = gae.paged_attention(q.expand(B, 2, D), k, v, table.expand(B, -1), lens, scale=math.log(2.0)).double()
+    _, kb, vb = _rows(k, v, table, 0, n)
+    ref = torch.softmax(q[0].double() @ kb[:, 0].T * math.log(2.0), 1) @ vb[:, 0]
+    share = 2 * (D + 4) * U * (below + 1) + (n + 8) * U + 2.0 ** -20 + (2.0 ** -17 if dtype != torch.float32 else 0)
+    step = n * 2.0 ** -38 * vb.max() if dtype == torch.float16 else 0.0
+    tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half the output's smallest step
+    err = (out - ref).abs()
+    assert (err <= (share + torch.finfo(dtype).eps / 2) * ref + step + tiny).all(), (err / ref).max().item()
