@@ -799,3 +799,26 @@ def test_attention_of_many_light_keys_beside_heavy_ones(gae, dtype, below):
     tiny = 2.0 ** -25 if dtype == torch.float16 else 0.0  # half the output's smallest step
     err = (out - ref).abs()
     assert (err <= (share + torch.finfo(dtype).eps / 2) * ref + step + tiny).all(), (err / ref).max().item()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_weights_are_the_same_every_time(gae, dtype):
+    """The weights that attention adds up, and those of a prompt, bit by bit, over split rows and short ones."""
+    g, page, B = _gen(46), 16, 3
+    k, v = _pools(700, 2, page, 128, dtype, g)
+    table = _table(B, 200, 700, g)
+    q = torch.randn(B, 8, 128, device="cuda", generator=g).to(dtype)
+    lens = torch.tensor([3200, 1501, 17], dtype=torch.int32, device="cuda")
+    w = torch.rand(B, 2, 3200, device="cuda", generator=g)
+    runs = []
+    for _ in range(6):
+        out = w.clone()
+        gae.paged_attention(q, k, v, table, lens, weights=w, weights_out=out)
+        runs.append(out)
+    assert not torch.equal(runs[0], w) and all(torch.equal(runs[0], r) for r in runs[1:])
+    if dtype == torch.float32:
+        return
+    qs, ks = (torch.randn(1, h, 900, 128, device="cuda", generator=g).to(dtype) for h in (4, 2))
+    lse = torch.full((1, 4, 900), 7.0, device="cuda")
+    runs = [gae.attention_key_weights(qs, ks, lse, causal=True) for _ in range(6)]
+    assert all(torch.equal(runs[0], r) for r in runs[1:])
