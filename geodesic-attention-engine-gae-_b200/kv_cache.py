@@ -400,7 +400,8 @@ class PagedKVCache:
             torch.zeros((batch, kv_heads, per * page_size), dtype=torch.float32, device=device)
             for _ in range(n_layers)]
         self.lengths = [0] * batch
-        self._reserved = None
+        self._reserved = None  # new tokens per sequence between reserve and commit
+        self._tokens = 0       # their number in the padded batch
 
     def reserve(self, tokens, counts=None):
         """Makes room for `tokens` new tokens of every sequence (counts: a list
@@ -412,7 +413,7 @@ class PagedKVCache:
         if longest > self.max_len:
             raise GAEError(1, f"PagedKVCache: {longest} positions, room for {self.max_len}")
         torch = _torch()
-        self._reserved = n
+        self._reserved, self._tokens = n, tokens
         if counts is None:
             torch.add(self.lens, tokens, out=self.next_lens)
         else:
@@ -423,6 +424,8 @@ class PagedKVCache:
         (T as reserved; a sequence's tokens beyond its count are dropped)."""
         if self._reserved is None:
             raise GAEError(1, "PagedKVCache: append without reserve")
+        if k_new.shape[2] != self._tokens:
+            raise GAEError(1, f"PagedKVCache: append of {k_new.shape[2]} tokens, {self._tokens} reserved")
         counts = None
         if any(c != k_new.shape[2] for c in self._reserved):
             counts = self.next_lens - self.lens

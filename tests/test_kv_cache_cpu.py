@@ -220,3 +220,18 @@ def test_cache_refusals(gae):
     assert b.evict() is None
     with pytest.raises(gae.GAEError):  # not empty any more
         gae.layer_stack_prefill([], torch.zeros(2, 1, 128, dtype=torch.bfloat16), b)
+
+
+def _cpu_cache(gae, **kw):
+    return gae.PagedKVCache(1, 2, 2, 64, 40, page_size=16, device="cpu", **kw)
+
+
+@pytest.mark.parametrize("counts", [None, [3, 1]])
+@pytest.mark.parametrize("given", [0, 1, 2, 4])
+def test_cache_append_takes_the_tokens_reserved(gae, counts, given):
+    """Fewer tokens than reserved would leave positions that no one wrote."""
+    c = _cpu_cache(gae)
+    c.reserve(3, counts)
+    k = torch.zeros(2, 2, given, 64, dtype=torch.bfloat16)
+    with pytest.raises(gae.GAEError, match=f"append of {given} tokens, 3 reserved"):
+        c.append(0, k, k)
