@@ -443,9 +443,13 @@ class PagedKVCache:
         attention(q, k, v, causal=True, return_lse=True)."""
         if self.weights is None:
             return
+        if self._reserved is None:
+            raise GAEError(1, "PagedKVCache: prompt weights without reserve")
         if any(self.lengths):
             raise GAEError(1, "PagedKVCache: prompt weights need an empty cache")
         T = q.shape[2]
+        if T != self._tokens or k.shape[2] != T:
+            raise GAEError(1, f"PagedKVCache: weights of {T} queries and {k.shape[2]} keys, {self._tokens} tokens reserved")
         torch = _torch()
         if any(c != T for c in self._reserved):  # queries beyond a sequence's own tokens weigh nothing
             pad = torch.arange(T, device=lse.device)[None] >= self.next_lens[:, None]

@@ -235,3 +235,15 @@ def test_cache_append_takes_the_tokens_reserved(gae, counts, given):
     k = torch.zeros(2, 2, given, 64, dtype=torch.bfloat16)
     with pytest.raises(gae.GAEError, match=f"append of {given} tokens, 3 reserved"):
         c.append(0, k, k)
+
+
+def test_cache_prompt_weights_take_the_tokens_reserved(gae):
+    c = _cpu_cache(gae, budget=20)
+    q = torch.zeros(2, 2, 3, 64, dtype=torch.bfloat16)
+    lse = torch.zeros(2, 2, 3)
+    with pytest.raises(gae.GAEError, match="prompt weights without reserve"):
+        c.add_prompt_weights(0, q, q, lse)
+    c.reserve(4)
+    for qq, kk in ((q, q), (torch.cat([q, q[:, :, :1]], 2), q)):
+        with pytest.raises(gae.GAEError, match="4 tokens reserved"):
+            c.add_prompt_weights(0, qq, kk, lse)
