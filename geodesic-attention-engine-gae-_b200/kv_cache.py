@@ -406,6 +406,8 @@ class PagedKVCache:
     def reserve(self, tokens, counts=None):
         """Makes room for `tokens` new tokens of every sequence (counts: a list
         of how many of them each sequence really has)."""
+        if tokens < 0:
+            raise GAEError(1, f"PagedKVCache: {tokens} tokens")
         n = [tokens] * self.batch if counts is None else [int(c) for c in counts]
         if len(n) != self.batch or any(not 0 <= c <= tokens for c in n):
             raise GAEError(1, f"PagedKVCache: counts must be {self.batch} numbers of [0, {tokens}]")

@@ -247,3 +247,13 @@ def test_cache_prompt_weights_take_the_tokens_reserved(gae):
     for qq, kk in ((q, q), (torch.cat([q, q[:, :, :1]], 2), q)):
         with pytest.raises(gae.GAEError, match="4 tokens reserved"):
             c.add_prompt_weights(0, qq, kk, lse)
+
+
+def test_cache_reserves_no_negative_tokens(gae):
+    c = _cpu_cache(gae)
+    c.reserve(7)
+    c.commit()
+    for counts in (None, [0, 0], [-5, -5]):
+        with pytest.raises(gae.GAEError):
+            c.reserve(-5, counts)
+    assert c.lengths == [7, 7] and c.next_lens.tolist() == [7, 7]
