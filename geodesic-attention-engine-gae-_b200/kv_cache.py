@@ -467,8 +467,11 @@ class PagedKVCache:
         self._reserved = None
 
     def refresh(self):
-        """Takes the host's lengths from the device (after replays; synchronises)."""
+        """Takes the host's lengths from the device (after replays; synchronises).
+        Raises where replays went past max_len: tokens beyond the pages are lost."""
         self.lengths = self.lens.tolist()
+        if max(self.lengths) > self.max_len:
+            raise GAEError(1, f"PagedKVCache: {max(self.lengths)} positions, room for {self.max_len}")
 
     def evict(self):
         """Brings every sequence back to the budget, if any is longer.  Returns

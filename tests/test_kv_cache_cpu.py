@@ -257,3 +257,13 @@ def test_cache_reserves_no_negative_tokens(gae):
         with pytest.raises(gae.GAEError):
             c.reserve(-5, counts)
     assert c.lengths == [7, 7] and c.next_lens.tolist() == [7, 7]
+
+
+def test_cache_refresh_tells_of_lost_tokens(gae):
+    c = _cpu_cache(gae)
+    c.lens.copy_(torch.tensor([40, 3]))
+    c.refresh()
+    assert c.lengths == [40, 3]
+    c.lens.copy_(torch.tensor([3, 41]))
+    with pytest.raises(gae.GAEError, match="41 positions, room for 40"):
+        c.refresh()
