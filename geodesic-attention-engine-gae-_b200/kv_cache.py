@@ -456,7 +456,9 @@ class PagedKVCache:
         if any(c != T for c in self._reserved):  # queries beyond a sequence's own tokens weigh nothing
             pad = torch.arange(T, device=lse.device)[None] >= self.next_lens[:, None]
             lse = lse.masked_fill(pad[:, None], -math.inf)
-        attention_key_weights(q, k, lse, causal=True, scale=scale, out=self.weights[layer][:, :, :T], accumulate=True)
+        w = self.weights[layer][:, :, :T]
+        n = w.shape[2]  # beyond the pages lies padding only
+        attention_key_weights(q[:, :, :n], k[:, :, :n], lse[:, :, :n], causal=True, scale=scale, out=w, accumulate=True)
 
     def commit(self):
         """The reserved tokens become part of the sequences."""

@@ -822,3 +822,20 @@ def test_weights_are_the_same_every_time(gae, dtype):
     lse = torch.full((1, 4, 900), 7.0, device="cuda")
     runs = [gae.attention_key_weights(qs, ks, lse, causal=True) for _ in range(6)]
     assert all(torch.equal(runs[0], r) for r in runs[1:])
+
+
+def test_a_prompt_padded_past_the_cache(gae):
+    """Right padding may be longer than the cache: its rows have no place, and no weight."""
+    B, H, D, g = 2, 4, 256, _gen(47)
+    layers = _layers(gae, 1, D, H, 512)
+    x = torch.randn(B, 80, D, device="cuda", generator=g).bfloat16()
+    counts, caches = [60, 33], []
+    for S, max_len in ((80, 60), (60, 60)):  # 64 positions of pages; the same prompt with and without the long padding
+        cache = gae.PagedKVCache(1, B, H, D // H, max_len, budget=40, recent=4)
+        y = gae.layer_stack_prefill(layers, x[:, :S].contiguous(), cache, counts)
+        caches.append((cache, y))
+    (a, ya), (b, yb) = caches
+    assert a.lengths == b.lengths == counts
+    for i, n in enumerate(counts):
+        assert torch.equal(ya[i, :n], yb[i, :n])
+        assert torch.equal(a.weights[0][i, :, :n], b.weights[0][i, :, :n]) and (a.weights[0][i, :, n:] == 0).all()
