@@ -498,5 +498,6 @@ class PagedKVCache:
         self.table[:, :n].copy_(self.spare)
         self.spare.copy_(first)
         self.lens.copy_(lens)
+        self.next_lens.copy_(lens)
         self.lengths = [min(a, self.budget) for a in self.lengths]
         return kept

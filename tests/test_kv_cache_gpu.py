@@ -839,3 +839,19 @@ def test_a_prompt_padded_past_the_cache(gae):
     for i, n in enumerate(counts):
         assert torch.equal(ya[i, :n], yb[i, :n])
         assert torch.equal(a.weights[0][i, :, :n], b.weights[0][i, :, :n]) and (a.weights[0][i, :, n:] == 0).all()
+
+
+def test_attend_after_an_eviction(gae):
+    """Between steps attend() sees what the cache holds, also right after an eviction."""
+    B, H, D, S, budget, g = 2, 4, 256, 100, 32, _gen(48)
+    layers = _layers(gae, 1, D, H, 512)
+    cache = gae.PagedKVCache(1, B, H, D // H, 128, budget=budget, recent=8)
+    gae.layer_stack_prefill(layers, torch.randn(B, S, D, device="cuda", generator=g).bfloat16(), cache)
+    cache.evict()
+    q = torch.randn(B, H, D // H, device="cuda", generator=g).bfloat16()
+    w = cache.weights[0].clone()
+    out = cache.attend(0, q)
+    for b, (k, v) in enumerate(_dense(cache, 0)):
+        p = torch.softmax(torch.einsum("hd,hnd->hn", q[b].double(), k) / math.sqrt(D // H), -1)
+        assert ((out[b].double() - torch.einsum("hn,hnd->hd", p, v)).abs() <= 2.0 ** -8 * v.abs().max()).all()
+    assert torch.equal(cache.weights[0][:, :, budget:], w[:, :, budget:])
