@@ -435,9 +435,14 @@ class PagedKVCache:
 
     def attend(self, layer, q, scale=None, out=None):
         """Attention of one new token per sequence, q [B, H, D], over everything
-        appended so far; adds up the keys' weights where there is a budget."""
-        return paged_attention(q, self.k[layer], self.v[layer], self.table, self.next_lens, scale=scale, out=out,
-                               weights=None if self.weights is None else self.weights[layer])
+        appended so far; adds up the keys' weights where there is a budget (a
+        sequence that reserve() counts no token of has no query: its keys' weights stay)."""
+        w = None if self.weights is None else self.weights[layer]
+        idle = [] if w is None else [(w[b], w[b].clone()) for b, c in enumerate(self._reserved or ()) if c == 0]
+        o = paged_attention(q, self.k[layer], self.v[layer], self.table, self.next_lens, scale=scale, out=out, weights=w)
+        for now, was in idle:
+            now.copy_(was)
+        return o
 
     def add_prompt_weights(self, layer, q, k, lse, scale=None):
         """Adds the weight that a prompt's queries put on its keys (an empty

@@ -855,3 +855,28 @@ def test_attend_after_an_eviction(gae):
         p = torch.softmax(torch.einsum("hd,hnd->hn", q[b].double(), k) / math.sqrt(D // H), -1)
         assert ((out[b].double() - torch.einsum("hn,hnd->hd", p, v)).abs() <= 2.0 ** -8 * v.abs().max()).all()
     assert torch.equal(cache.weights[0][:, :, budget:], w[:, :, budget:])
+
+
+def test_a_sequence_without_a_new_token_draws_no_weights(gae):
+    """In a step that only some sequences take part in, the others' row of q is padding: what it holds
+    reaches neither their keys' weights nor anyone else's output."""
+    B, H, Hkv, D, g = 3, 4, 2, 64, _gen(49)
+    cache = gae.PagedKVCache(1, B, Hkv, D, 64, budget=64)
+    rows = torch.randn(B, Hkv, 40, D, device="cuda", generator=g).bfloat16()
+    cache.reserve(40, [40, 17, 5])
+    cache.append(0, rows, rows)
+    cache.commit()
+    cache.weights[0].copy_(torch.rand(cache.weights[0].shape, device="cuda", generator=g))
+    was = cache.weights[0].clone()
+    q = torch.randn(B, H, D, device="cuda", generator=g).bfloat16()
+    q[1] = math.nan
+    cache.reserve(1, [1, 0, 1])
+    cache.append(0, rows[:, :, :1], rows[:, :, :1])
+    out = cache.attend(0, q)
+    cache.commit()
+    assert cache.lens.tolist() == cache.lengths == [41, 17, 6]
+    assert torch.equal(cache.weights[0][1], was[1])
+    assert out[0].isfinite().all() and out[2].isfinite().all()
+    for b, n in ((0, 41), (2, 6)):
+        drawn = (cache.weights[0][b] - was[b]).double()
+        assert ((drawn.sum(-1) - H // Hkv).abs() <= 1e-4).all() and (drawn[:, n:] == 0).all()
