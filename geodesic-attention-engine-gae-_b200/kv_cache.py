@@ -370,9 +370,10 @@ class PagedKVCache:
     held for that).
 
     reserve, append, attend and commit launch on the current stream and may be
-    captured into a CUDA graph; `lengths`, the host's count that the capacity
-    check and evict() go by, does not move on a replay: refresh() reads it back
-    from the device."""
+    captured into a CUDA graph (a replay takes the counts of the capture);
+    `lengths`, the host's count that the capacity check and evict() go by, moves
+    once for the capture and not on a replay: refresh() reads it back from the
+    device."""
 
     def __init__(self, n_layers, batch, kv_heads, head_dim, max_len, *, page_size=16, dtype=None, device="cuda",
                  budget=None, recent=0):
@@ -418,6 +419,9 @@ class PagedKVCache:
         self._reserved, self._tokens = n, tokens
         if counts is None:
             torch.add(self.lens, tokens, out=self.next_lens)
+        elif self.lens.is_cuda and torch.cuda.is_current_stream_capturing():  # which takes no copy from the host
+            for b, c in enumerate(n):
+                torch.add(self.lens[b: b + 1], c, out=self.next_lens[b: b + 1])
         else:
             torch.add(self.lens, torch.tensor(n, dtype=torch.int32, device=self.lens.device), out=self.next_lens)
 

@@ -880,3 +880,34 @@ def test_a_sequence_without_a_new_token_draws_no_weights(gae):
     for b, n in ((0, 41), (2, 6)):
         drawn = (cache.weights[0][b] - was[b]).double()
         assert ((drawn.sum(-1) - H // Hkv).abs() <= 1e-4).all() and (drawn[:, n:] == 0).all()
+
+
+def test_a_ragged_step_in_a_graph(gae):
+    """reserve(counts) may be captured: a step that only some sequences take part in, replayed."""
+    B, H, D, g = 3, 2, 64, _gen(50)
+    rows = torch.randn(B, H, 2, D, device="cuda", generator=g).bfloat16()
+    q = torch.randn(B, H, D, device="cuda", generator=g).bfloat16()
+    eager, graphed = (gae.PagedKVCache(1, B, H, D, 64, budget=64) for _ in range(2))
+
+    def step(cache):
+        cache.reserve(2, [2, 0, 1])
+        cache.append(0, rows, rows)
+        out = cache.attend(0, q)
+        cache.commit()
+        return out
+
+    want = [step(eager) for _ in range(5)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(graphed)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(graphed)
+    for t in range(1, 5):
+        graph.replay()
+        assert torch.equal(out, want[t]), t
+    graphed.refresh()
+    assert graphed.lengths == eager.lengths == [10, 0, 5]
+    assert torch.equal(eager.weights[0], graphed.weights[0])
