@@ -267,3 +267,86 @@ def test_cache_refresh_tells_of_lost_tokens(gae):
     c.lens.copy_(torch.tensor([3, 41]))
     with pytest.raises(gae.GAEError, match="41 positions, room for 40"):
         c.refresh()
+
+
+def test_python_refusals_name_their_reason(gae):
+    """Each check of the wrappers by the words of its own refusal: a call that slipped through one would
+    end at the device check, whose words are others."""
+    z = torch.zeros
+    half = dict(dtype=torch.bfloat16)
+    k = z(4, 2, 16, 64, **half)
+    table, ints = z(3, 2, dtype=torch.int32), z(3, dtype=torch.int32)
+    new, q, w = z(3, 2, 5, 64, **half), z(3, 4, 64, **half), z(3, 2, 32)
+    wide = z(3, 4, dtype=torch.int32)
+
+    def call(fn, base, **s):
+        return lambda: fn(**{**base, **s})
+
+    append = lambda **s: call(gae.paged_append, dict(k_new=new, v_new=new, k_pages=k, v_pages=k, page_table=table,  # noqa: E731
+                                                     start=ints), **s)
+    attend = lambda **s: call(gae.paged_attention, dict(q=q, k_pages=k, v_pages=k, page_table=table, seq_lens=ints), **s)  # noqa: E731
+    evict = lambda **s: call(gae.paged_evict, dict(k_pages=k, v_pages=k, page_table=table, seq_lens=ints, weights=w,  # noqa: E731
+                                                   dst_table=z(3, 1, dtype=torch.int32), keep=8), **s)
+    keys = lambda **s: call(gae.attention_key_weights, dict(q=z(1, 2, 8, 64), k=z(1, 2, 8, 64), lse=z(1, 2, 8)), **s)  # noqa: E731
+    for c, why in [
+        (append(k_new=new.float(), v_new=new.float()), "new rows and pages must share a dtype"),
+        (append(v_new=new.float()), "new rows and pages must share a dtype"),
+        (append(v_new=new[:, :, :3]), r"must be \[batch, kv_heads, tokens, head_dim\]"),
+        (append(k_new=new[0], v_new=new[0]), r"must be \[batch, kv_heads, tokens, head_dim\]"),
+        (append(k_new=z(3, 3, 5, 64, **half), v_new=z(3, 3, 5, 64, **half)), "differ in heads or head_dim"),
+        (append(k_new=new[..., :32], v_new=new[..., :32]), "differ in heads or head_dim"),
+        (append(k_new=z(3, 2, 64, 5, **half).transpose(2, 3)), "new rows must have a contiguous head_dim"),
+        (append(start=ints.long()), r"start must be contiguous int32 \[batch\]"),
+        (append(start=z(6, dtype=torch.int32)[::2]), r"start must be contiguous int32 \[batch\]"),
+        (append(counts=ints[:2]), r"counts must be contiguous int32 \[batch\]"),
+        (append(counts=ints.float()), r"counts must be contiguous int32 \[batch\]"),
+        (append(page_table=table.long()), r"page_table must be int32 \[batch, max_pages\]"),
+        (append(page_table=table[:2]), r"page_table must be int32 \[batch, max_pages\]"),
+        (append(page_table=table[0]), r"page_table must be int32 \[batch, max_pages\]"),
+        (append(page_table=wide[:, ::2]), "page_table must have contiguous rows"),
+        (append(v_pages=k[:3]), r"must be \[num_pages, kv_heads, page_size, head_dim\]"),
+        (append(k_pages=k[0], v_pages=k[0]), r"must be \[num_pages, kv_heads, page_size, head_dim\]"),
+        (append(v_pages=k.half()), "k_pages and v_pages must share a dtype"),
+        (append(k_pages=z(4, 2, 64, 16, **half).transpose(2, 3)), "pages must have a contiguous head_dim"),
+        (append(k_pages=k.long(), v_pages=k.long()), "unsupported dtype"),
+        (attend(q=q[0]), r"q must be \[batch, heads, head_dim\]"),
+        (attend(q=q.float()), "differ in head_dim or dtype"),
+        (attend(q=q[..., :32]), "differ in head_dim or dtype"),
+        (attend(q=z(3, 64, 4, **half).transpose(1, 2)), "q must have a contiguous head_dim"),
+        (attend(seq_lens=ints[:1]), r"seq_lens must be contiguous int32 \[batch\]"),
+        (attend(seq_lens=ints.long()), r"seq_lens must be contiguous int32 \[batch\]"),
+        (attend(page_table=wide[:, ::2]), "page_table must have contiguous rows"),
+        (attend(page_table=table.t()), r"page_table must be int32 \[batch, max_pages\]"),
+        (attend(weights=w[..., :31]), r"weights must be fp32 \[3, 2, >= 32\]"),
+        (attend(weights=w.double()), r"weights must be fp32 \[3, 2, >= 32\]"),
+        (attend(weights=w[:, :1]), r"weights must be fp32 \[3, 2, >= 32\]"),
+        (attend(weights=z(3, 2, 64)[..., ::2]), "weights must have contiguous rows"),
+        (attend(weights=w, weights_out=w[..., :31]), r"weights_out must be fp32 \[3, 2, >= 32\]"),
+        (attend(weights_out=w), "weights_out without weights"),
+        (attend(lse=z(3, 3)), r"lse must be contiguous fp32 \[batch, heads\]"),
+        (attend(lse=z(4, 3).t()), r"lse must be contiguous fp32 \[batch, heads\]"),
+        (attend(lse=z(3, 4, **half)), r"lse must be contiguous fp32 \[batch, heads\]"),
+        (attend(out=q.float()), "out must be like q"),
+        (attend(out=q[:2]), "out must be like q"),
+        (attend(out=z(3, 64, 4, **half).transpose(1, 2)), "out must be like q"),
+        (evict(weights=w[:, :1]), r"weights must be fp32 \[3, 2, >= 0\]"),
+        (evict(weights=w.half()), r"weights must be fp32 \[3, 2, >= 0\]"),
+        (evict(dst_table=z(2, 1, dtype=torch.int32)), r"dst_table must be int32 \[batch, max_pages\]"),
+        (evict(seq_lens=ints.float()), r"seq_lens must be contiguous int32 \[batch\]"),
+        (evict(keep=0), "keep must be positive"),
+        (keys(q=z(2, 8, 64)), r"must be \[batch, heads, seq, head_dim\]"),
+        (keys(k=z(1, 2, 8, 32)), "differ in batch, head_dim or dtype"),
+        (keys(k=z(1, 2, 8, 64).half()), "differ in batch, head_dim or dtype"),
+        (keys(k=z(2, 2, 8, 64)), "differ in batch, head_dim or dtype"),
+        (keys(q=z(1, 2, 64, 8).transpose(2, 3)), "q and k must have a contiguous head_dim"),
+        (keys(lse=z(1, 2, 7)), r"lse must be fp32 \[1, 2, >= 8\]"),
+        (keys(lse=z(1, 2, 9)), r"lse must be \[batch, heads, seq_q\]"),
+        (keys(lse=z(1, 2, 16)[..., ::2]), "lse must have contiguous rows"),
+        (keys(accumulate=True), "accumulate needs out"),
+        (keys(out=z(1, 2, 7)), r"out must be \[1, 2, 8\]"),
+        # all in order but for the device
+        (append(), "k_pages is on cpu"), (append(counts=ints), "k_pages is on cpu"), (attend(), "q is on cpu"),
+        (attend(weights=w), "q is on cpu"), (evict(), "k_pages is on cpu"), (keys(), "q is on cpu"),
+    ]:
+        with pytest.raises(gae.GAEError, match=why):
+            c()
