@@ -284,6 +284,8 @@ gae_status gae_key_weights(const gae_key_weights_args *a, void *stream) {
     if (a->batch * a->heads > 65535) return fail(GAE_ERR_UNSUPPORTED, "batch*heads > 65535");
     if (a->seq_q > kMaxPositions || a->seq_kv > kMaxPositions)
         return fail(GAE_ERR_UNSUPPORTED, "sequence longer than 2^30");
+    if (a->heads / a->kv_heads * ((a->seq_q + 127) / 128) > INT32_MAX)  // a CTA counts its query tiles in an int
+        return fail(GAE_ERR_UNSUPPORTED, "more than 2^31 - 1 query tiles to a key head");
     if (!(a->scale >= 0.f)) return fail(GAE_ERR_UNSUPPORTED, "negative or NaN scale");
     if (a->seq_kv == 0) return GAE_OK;
     if (!a->out || (a->seq_q > 0 && (!a->q || !a->k || !a->lse)))

@@ -350,3 +350,17 @@ def test_python_refusals_name_their_reason(gae):
     ]:
         with pytest.raises(gae.GAEError, match=why):
             c()
+
+
+def test_key_weights_query_tiles_fit_an_int(gae):
+    """2^23 query tiles times 256 heads on one key head are 2^31: one too many."""
+    L, n = gae.lib(), 1 << 30
+    wide = dict(heads=256, kv_heads=1, seq_q=n, q_stride=(0, 0, 64), lse_stride=(0, 0), out_stride=(16, 16))
+    assert L.gae_key_weights(C.byref(_args(gae.KeyWeightsArgs, KEYS, **wide)), None) == UNSUPPORTED
+    assert b"query tiles" in _last_error(L)
+
+
+def _last_error(L):
+    buf = C.create_string_buffer(512)
+    L.gae_last_error(buf, 512)
+    return buf.value
