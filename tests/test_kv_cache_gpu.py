@@ -911,3 +911,58 @@ def test_a_ragged_step_in_a_graph(gae):
     graphed.refresh()
     assert graphed.lengths == eager.lengths == [10, 0, 5]
     assert torch.equal(eager.weights[0], graphed.weights[0])
+
+
+def test_broadcast_operands(gae):
+    """Strides of 0: one q for all sequences, one lse row for all heads, one prompt for all of the batch."""
+    g, B, Hkv, page, D = _gen(51), 3, 2, 16, 64
+    k, v = _pools(40, Hkv, page, D, torch.bfloat16, g)
+    table = _table(1, 12, 40, g).expand(B, 12)
+    q = torch.randn(1, 1, D, device="cuda", generator=g).bfloat16().expand(B, 6, D)
+    lens = torch.tensor([1, 100, 192], dtype=torch.int32, device="cuda")
+    _check_attention(gae, q, k, v, table, lens)
+    qk = torch.randn(1, 1, 200, D, device="cuda", generator=g).bfloat16().expand(2, 4, 200, D)
+    kk = torch.randn(1, 1, 300, D, device="cuda", generator=g).bfloat16().expand(2, 2, 300, D)
+    lse = torch.full((1, 1, 200), 6.0, device="cuda").expand(2, 4, 200)
+    w = gae.attention_key_weights(qk, kk, lse, causal=True, q_offset=100)
+    _check_keys(gae, qk, kk, lse, w, True, 100)
+    rows = torch.randn(1, 1, 1, D, device="cuda", generator=g).bfloat16().expand(B, Hkv, 3, D)
+    own = _table(B, 12, 40, g)
+    start = torch.tensor([0, 15, 189], dtype=torch.int32, device="cuda")
+    gae.paged_append(rows, rows, k, v, own, start)
+    for b, s in enumerate(start.tolist()):
+        for t in range(s, s + 3):
+            assert torch.equal(k[own[b, t // page].long(), :, t % page], rows[0, :, 0])
+
+
+def test_two_graphs_of_one_model_at_once(gae):
+    """Two captured runs of the same sizes, replayed together on two streams: each has its own workspace."""
+    g, Hkv, page, D, M = _gen(52), 2, 16, 128, 100
+    runs = []
+    for i in range(2):
+        k, v = _pools(2 * M, Hkv, page, D, torch.bfloat16, g)
+        table = _table(2, M, 2 * M, g)
+        q = torch.randn(2, 8, D, device="cuda", generator=g).bfloat16()
+        lens = torch.tensor([1600, 900 + i], dtype=torch.int32, device="cuda")
+        w = torch.rand(2, Hkv, M * page, device="cuda", generator=g)
+        qk, kk = (torch.randn(1, h, 1000, D, device="cuda", generator=g).bfloat16() for h in (4, 2))
+        lse = torch.full((1, 4, 1000), 7.0, device="cuda")
+        graph, stream, wo = torch.cuda.CUDAGraph(), torch.cuda.Stream(), w.clone()
+        call = lambda: (*gae.paged_attention(q, k, v, table, lens, return_lse=True, weights=w, weights_out=wo),  # noqa: B023,E731
+                        gae.attention_key_weights(qk, kk, lse, causal=True))  # noqa: B023
+        want = [t.clone() for t in (*call(), wo)]
+        _check_attention(gae, q, k, v, table, lens, got=want[:2])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            got = (*call(), wo)
+        runs.append((graph, stream, got, want, (k, v, table, q, lens, w, qk, kk, lse)))  # what the graph reads lives on
+    for _ in range(20):
+        for graph, stream, got, _, kept in runs:
+            with torch.cuda.stream(stream):
+                for t in got[:3]:
+                    t.fill_(-1)
+                got[3].copy_(kept[5])  # entries behind a sequence's length are not written
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, _, got, want, _ in runs:
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
