@@ -19,7 +19,10 @@
 // What bounds it: one exponential per score.  The MUFU gives 16 a cycle and
 // SM, a 128 x 128 tile takes it 1024 cycles where the products at head_dim 128
 // take 512.  All exponentials are the MUFU's, which keeps NaN, gives +inf from
-// 2^128 on and 0 below 2^-126 whatever column a query stands in.
+// 2^128 on and 0 below 2^-126 whatever column a query stands in.  A polynomial
+// on the FMA pipe for every third pair took as long within 2% and had none of
+// that.  8192 x 8192 causal, 16 heads x 128: 182 us, MUFU 78% and tensor pipe 40%
+// busy; 200 x 32768, 32 heads on 8, 128: 93 us, 66% and 37%.
 #pragma once
 #include <cfloat>
 

@@ -81,7 +81,7 @@ PagedWs paged_ws(int64_t B, int64_t H, int64_t Hkv, int64_t D, int64_t cap, bool
 
 // How many CTAs share a pair of key tiles' queries: enough to fill the GPU (two
 // CTAs to an SM) as long as each is left with 4 query tiles (1000 x 1000, 24
-// heads x 64: 12.5 us replayed from a graph with 4, 12.7 with 2, 15.9 with 8 and
+// heads x 64: 13.1 us replayed from a graph with 4, 13.2 with 2, 16.8 with 8 and
 // thus one launch).  (Four times as many, so that a causal mask's long units end
 // together, gained nothing: 178 against 180 us at 8192 x 8192, 16 heads.)
 int key_weights_splits(int64_t B, int64_t H, int64_t Hkv, int64_t Nq, int64_t Nkv) {

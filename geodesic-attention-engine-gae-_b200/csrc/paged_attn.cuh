@@ -3,9 +3,9 @@
 //
 //   o = sum_t softmax_t(scale <q, k_t>) v_t,  t < len,  per (sequence, head)
 //
-// Every cached row is read once for all query heads that share it, so the work
-// is bound by the cache's bytes; the kernels are built to keep enough of them
-// in flight.  A row (sequence, key head, group of up to 16 query heads) is cut
+// Every cached row is read once for up to 16 query heads that share it (8 in
+// fp32; once for each such group where more do), so the work is bound by the
+// cache's bytes; the kernels are built to keep enough of them in flight.  A row (sequence, key head, group of up to 16 query heads) is cut
 // into tiles of kKeys positions to a warp and the tiles of all rows, in order, are
 // dealt in equal runs to a grid that fills the GPU once, whatever the lengths
 // are: they are read on the device, so a captured graph stays balanced when

@@ -222,7 +222,8 @@ def paged_attention(q, k_pages, v_pages, page_table, seq_lens, *, scale=None, ou
     """Attention of one new token per sequence: q [B, H, D] over the first
     seq_lens[b] cached positions (int32 [B]); H a multiple of the pages' heads.
     bf16/f16/f32, any head_dim <= 256 in 16-byte multiples.  An empty sequence
-    gives 0 and lse -inf.
+    gives 0 and lse -inf; an infinite value among a sequence's own gives NaN in
+    16 bits (probabilities are held as the sum of two numbers).
 
     weights (fp32 [B, Hkv, >= the page table's positions]) asks for the keys'
     attention weight: weights_out = weights + the softmax summed over each key
@@ -281,7 +282,8 @@ def attention_key_weights(q, k, lse, *, causal=False, scale=None, q_offset=0, kv
     sum over the queries that see the key (and the query heads of its key head)
     of exp(scale * <q, k> - lse).  q [B, H, Nq, D], k [B, Hkv, Nkv, D] (bf16/f16,
     head_dim 64/128, strided views allowed), lse [B, H, Nq] as attention(...,
-    return_lse=True) gives it (contiguous rows).  A window of a prompt's last
+    return_lse=True) gives it (contiguous rows; a query whose lse is -inf adds
+    nothing, whatever it holds).  A window of a prompt's last
     queries is q[:, :, -n:], lse[:, :, -n:] with q_offset = N - n.  out may be a
     view of a cache's weights; accumulate=True adds to it."""
     what = "attention_key_weights"
