@@ -726,13 +726,30 @@ class Gpt2Layer:
         h = layernorm_rows(x1, w["ln2_gamma"], w["ln2_beta"], self.eps)
         return linear(linear(h, w["w_fc"], w["b_fc"], gelu=True), w["w_fc2"], w["b_fc2"], res=x1)
 
+    def _cached(self, what, x, dims, cache, layer):
+        """x, refused before anything is
+        launched or written where it does not fit this layer and the cache's."""
+        torch = _torch()
+        if x.dim() != dims or x.dtype != torch.bfloat16 or x.shape[0] != cache.batch or x.shape[-1] != self.d_model:
+            shape = f"[{cache.batch}, {'S, ' if dims == 3 else ''}{self.d_model}]"
+            raise GAEError(1, f"{what}: x must be bf16 {shape}")
+        if not 0 <= layer < len(cache.k):
+            raise GAEError(1, f"{what}: layer {layer} of a cache of {len(cache.k)}")
+        k = cache.k[layer]
+        if (k.shape[1], k.shape[3]) != (self.heads, self.d_model // self.heads) or k.dtype != torch.bfloat16:
+            raise GAEError(1, f"{what}: the cache must be bf16 with {self.heads} heads of {self.d_model // self.heads}")
+        if not x.is_cuda or x.get_device() != torch.cuda.current_device():
+            raise GAEError(1, f"{what}: x must be on the current CUDA device")
+        return x
+
     def prefill(self, x, cache, layer):
         """forward() of a prompt that also writes its keys and values (and, with a
         budget, their weights) to layer `layer` of a PagedKVCache whose reserve()
-        has made room for it.  x: bf16 [B, S, d_model] contiguous, right-padded;
-        the cache's sequences have to be empty (a prompt attends to itself alone)."""
+        has made room for it.  x: bf16 [B, S, d_model] contiguous, right-padded; the cache's
+        sequences have to be empty (a prompt attends to itself alone)."""
         if any(cache.lengths):
             raise GAEError(1, "prefill: the cache is not empty")
+        x = self._cached("prefill", x, 3, cache, layer)
         B, S, D = x.shape
         w, x = self.w, x.reshape(B * S, D)
         h = layernorm_rows(x, w["ln1_gamma"], w["ln1_beta"], self.eps)
@@ -746,7 +763,7 @@ class Gpt2Layer:
     def decode(self, x, cache, layer):
         """One new token per sequence, x bf16 [B, d_model], over layer `layer` of
         the cache, which takes in the token's key and value first."""
-        w = self.w
+        w, x = self.w, self._cached("decode", x, 2, cache, layer)
         h = layernorm_rows(x, w["ln1_gamma"], w["ln1_beta"], self.eps)
         q, k, v = self._heads(linear(h, w["w_qkv"], w["b_qkv"]), x.shape[0])
         cache.append(layer, k.unsqueeze(2), v.unsqueeze(2))

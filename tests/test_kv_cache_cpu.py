@@ -364,3 +364,23 @@ def _last_error(L):
     buf = C.create_string_buffer(512)
     L.gae_last_error(buf, 512)
     return buf.value
+
+
+def test_layer_refuses_what_does_not_fit_it(gae):
+    """Before a kernel reads a row as wide as x from parameters of another width, or a row is written."""
+    z = lambda *s, t=torch.bfloat16: torch.zeros(*s, dtype=t)  # noqa: E731
+    layer = gae.Gpt2Layer.random(256, 4, 512, device="cpu")
+    new = lambda heads=4, hd=64, t=torch.bfloat16: gae.PagedKVCache(1, 2, heads, hd, 40, dtype=t, device="cpu")  # noqa: E731
+    for x, cache, i, why in [
+        (z(2, 512), new(), 0, r"x must be bf16 \[2, 256\]"), (z(2, 255), new(), 0, r"x must be bf16 \[2, 256\]"),
+        (z(3, 256), new(), 0, r"x must be bf16 \[2, 256\]"), (z(256), new(), 0, r"x must be bf16 \[2, 256\]"),
+        (z(2, 256, t=torch.float32), new(), 0, r"x must be bf16 \[2, 256\]"),
+        (z(2, 256), new(), 1, "layer 1 of a cache of 1"), (z(2, 256), new(2), 0, "4 heads of 64"),
+        (z(2, 256), new(4, 32), 0, "4 heads of 64"), (z(2, 256), new(t=torch.float16), 0, "4 heads of 64"),
+        (z(2, 256), new(), 0, "x must be on the current CUDA device"),
+    ]:
+        cache.reserve(1)
+        with pytest.raises(gae.GAEError, match=why):
+            layer.decode(x, cache, i)
+        with pytest.raises(gae.GAEError, match=why.replace("[2, 256", "[2, S, 256")):
+            layer.prefill(x.unsqueeze(1), cache, i)
