@@ -727,7 +727,7 @@ class Gpt2Layer:
         return linear(linear(h, w["w_fc"], w["b_fc"], gelu=True), w["w_fc2"], w["b_fc2"], res=x1)
 
     def _cached(self, what, x, dims, cache, layer):
-        """x, refused before anything is
+        """x as the kernels read it (contiguous rows), refused before anything is
         launched or written where it does not fit this layer and the cache's."""
         torch = _torch()
         if x.dim() != dims or x.dtype != torch.bfloat16 or x.shape[0] != cache.batch or x.shape[-1] != self.d_model:
@@ -740,18 +740,18 @@ class Gpt2Layer:
             raise GAEError(1, f"{what}: the cache must be bf16 with {self.heads} heads of {self.d_model // self.heads}")
         if not x.is_cuda or x.get_device() != torch.cuda.current_device():
             raise GAEError(1, f"{what}: x must be on the current CUDA device")
-        return x
+        return x.contiguous()
 
     def prefill(self, x, cache, layer):
         """forward() of a prompt that also writes its keys and values (and, with a
         budget, their weights) to layer `layer` of a PagedKVCache whose reserve()
-        has made room for it.  x: bf16 [B, S, d_model] contiguous, right-padded; the cache's
+        has made room for it.  x: bf16 [B, S, d_model], right-padded; the cache's
         sequences have to be empty (a prompt attends to itself alone)."""
         if any(cache.lengths):
             raise GAEError(1, "prefill: the cache is not empty")
         x = self._cached("prefill", x, 3, cache, layer)
         B, S, D = x.shape
-        w, x = self.w, x.reshape(B * S, D)
+        w, x = self.w, x.view(B * S, D)
         h = layernorm_rows(x, w["ln1_gamma"], w["ln1_beta"], self.eps)
         q, k, v = (t.transpose(1, 2) for t in self._heads(linear(h, w["w_qkv"], w["b_qkv"]), B, S))
         att, lse = attention(q, k, v, causal=True, return_lse=True)

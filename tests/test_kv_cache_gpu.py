@@ -966,3 +966,16 @@ def test_two_graphs_of_one_model_at_once(gae):
     torch.cuda.synchronize()
     for _, _, got, want, _ in runs:
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_decode_and_prefill_of_slices(gae):
+    """The last hidden states of a prompt, and every second token of a longer one, taken as they lie."""
+    B, H, D, S, g = 3, 4, 256, 20, _gen(53)
+    layers = _layers(gae, 2, D, H, 512)
+    x = torch.randn(B, 2 * S, D, device="cuda", generator=g).bfloat16()
+    got = []
+    for take in (lambda t: t, lambda t: t.contiguous()):
+        cache = gae.PagedKVCache(2, B, H, D // H, 64, budget=64)
+        y = gae.layer_stack_prefill(layers, take(x[:, ::2]), cache)
+        got.append((y, gae.layer_stack_decode(layers, take(y[:, -1]), cache), *cache.weights))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
